@@ -27,7 +27,7 @@ _lib = C.CDLL(LIB_PATH)
 
 vp, i32, i64, f32, sz = C.c_void_p, C.c_int, C.c_longlong, C.c_float, C.c_size_t
 
-ABI = 103           # csmri_version() of the library these structures mirror (103: csmri_adam_dev_lr; 102: csmri_gconv_desc.out_q .. out_amax)
+ABI = 104           # csmri_version() of the library these structures mirror (104: csmri_ln_*, csmri_act8_*, csmri_mx4_*; 103: csmri_adam_dev_lr; 102: csmri_gconv_desc.out_q .. out_amax)
 _lib.csmri_version.restype = C.c_int
 if _lib.csmri_version() != ABI:
   raise RuntimeError('%s reports ABI %d, this binding is for %d: rebuild the library (python __graft_entry__.py)'
@@ -218,6 +218,21 @@ _SIGS = {
     'csmri_bucket_pack_bf16': (i32, [vp, i64, vp, i64, vp]),
     'csmri_bucket_reduce': (i32, [vp, i32, i64, vp, vp]),
     'csmri_bucket_unpack_bf16': (i32, [vp, i64, vp, vp]),
+    'csmri_ln_fwd': (i32, [i32, vp, i32, vp, i32, i64, i32, i32, vp, vp, f32, f32, vp, vp, vp, vp, vp]),
+    'csmri_ln_bwd_rows': (i32, [i64, i32]),
+    'csmri_ln_bwd': (i32, [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, vp, i32, i64, i32, i32, vp, f32, f32, vp, vp, vp,
+                           i32, vp]),
+    'csmri_act8_save': (i32, [i32, vp, i32, i64, i32, vp, vp, vp]),
+    'csmri_act8_restore': (i32, [vp, vp, i64, i32, i32, vp, i32, vp]),
+    'csmri_act8_wgrad_splits': (i32, [i64, i32, i32]),
+    'csmri_act8_wgrad_slab_bytes': (sz, [i32, i32, i32]),
+    'csmri_act8_wgrad': (i32, [i32, vp, i32, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp]),
+    'csmri_mx4_code_bytes': (i32, [i32]),
+    'csmri_mx4_scale_bytes': (i32, [i32]),
+    'csmri_mx4_quantize': (i32, [i32, vp, i32, i64, i32, vp, vp, vp]),
+    'csmri_mx4_dequantize': (i32, [vp, vp, i64, i32, i32, vp, i32, vp]),
+    'csmri_mx4_linear_work_bytes': (sz, [i32, i64, i32]),
+    'csmri_mx4_linear': (i32, [i32, vp, i32, vp, i64, i32, vp, vp, i32, vp, f32, vp, i32, i32, vp, vp]),
     'csmri_fill_f32': (i32, [vp, i64, f32, vp]),
     'csmri_cast': (i32, [vp, i32, vp, i32, i64, vp]),
     'csmri_copy_channels': (i32, [vp, i32, i32, i32, vp, i32, i32, i32, i64, vp]),

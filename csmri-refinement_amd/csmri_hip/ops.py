@@ -16,6 +16,7 @@ from . import lib
 from .lib import F32, BF16, BORDER_ZERO, BORDER_REFLECT
 
 FP8 = 2               # CSMRI_FP8: OCP e4m3fn operands of the fp8 convolution variant
+MX4 = 4               # CSMRI_MX4: microscaled 4-bit rows, an operand of csmri_mx4_linear
 
 _EPOCH = [0]          # bumped whenever trainable weights change (optimizer step / load)
 
@@ -160,6 +161,9 @@ class ConvLayer(object):
     self.train_weights = True               # False: skip wgrad (e.g. D during the G backward)
     self.fp8 = False                        # True: forward products on fp8 operands where the shape allows
     self._pack8 = None
+    self.mx4 = False                        # True: forward products on 4-bit operands where the shape allows (1 x 1)
+    self._pack4 = None
+    self.keep8 = False                      # True: the layer's input is kept for its weight gradient in 8 bits
 
   # -- packs ---------------------------------------------------------------
   def _pack(self, mode):
@@ -216,6 +220,26 @@ class ConvLayer(object):
              scales.data_ptr() + 4, stream())
     self._pack8 = (epoch, q, kp.value, scales)
     return q, kp.value, scales
+
+  def pointwise(self):
+    """A 1 x 1 stride-1 convolution without padding or upsampling: a matrix product over pixels."""
+    return self.kh == self.kw == 1 and self.stride == 1 and not any(self.pads) and not self.upsample
+
+  def mx4_ok(self, x1):
+    return self.mx4 and x1 is None and self.pointwise()
+
+  def _pack_mx4(self):
+    """The layer's weights as 4-bit rows of ``cin_p`` channels (csmri_mx4_quantize)."""
+    epoch = _weight_epoch(self)
+    ent = self._pack4
+    if ent is not None and ent[0] == epoch and ent[1].codes.device == self.weight.device:
+      return ent[1]
+    w = self.weight.detach().reshape(self.cout, self.cin)
+    if self.cin_p != self.cin:
+      w = torch.nn.functional.pad(w, (0, self.cin_p - self.cin))
+    q = mx4_quantize(w, ent[1] if ent is not None and ent[1].codes.device == self.weight.device else None)
+    self._pack4 = (epoch, q)
+    return q
 
   def bias_padded(self):
     if self.bias is None:
@@ -397,6 +421,235 @@ def quantize_fp8(x, amax=None):
   return q, scales
 
 
+# ----------------------------------------------------------------------------
+# block-scaled formats: kept activations (8 bits), 4-bit rows, layer norm
+# ----------------------------------------------------------------------------
+# These take tensors [..., C] of any leading shape, their last axis the channels of a pixel (C a multiple of 8, pad
+# channels zero), strided pixels included; what the kernels cannot address (a strided channel axis, a pointer or pixel
+# stride that is no multiple of 16 bytes) is copied first.  They launch on the current stream of the tensor's device.
+
+
+def _pixels(t):
+  """(tensor, pixels, channels, pixel stride) of ``t`` [..., C]."""
+  _need_gpu(t)
+  dt_of(t)
+  c = t.shape[-1] if t.dim() else 0
+  if c == 0 or c % 8:
+    raise ValueError('csmri_hip: the channel axis has to be a multiple of 8 (got shape %s)' % (tuple(t.shape),))
+  n = t.numel() // c
+  ps, span, ok = c, 0, t.stride(-1) == 1
+  for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    if size == 1 or n == 0:
+      continue
+    if span == 0:
+      ps, span = st, st * size
+    else:
+      ok, span = ok and st == span, span * size
+  es = t.element_size()
+  if not ok or ps < c or ps * es % 16 or t.data_ptr() % 16:
+    t, ps = t.contiguous(), c
+    if t.data_ptr() % 16:
+      t = t.clone()
+  return t, n, c, ps
+
+
+def _on_device_of(t, *others):
+  for o in others:
+    if o is not None and o.device != t.device:
+      raise RuntimeError('csmri_hip: operands on %s and %s' % (t.device, o.device))
+  return torch.cuda.device(t.device)
+
+
+def _vector(t, n, what):
+  if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
+    raise ValueError('csmri_hip: %s has to be fp32 [%d], got %s %s' % (what, n, t.dtype, tuple(t.shape)))
+  return t.detach().contiguous()
+
+
+class Act8(object):
+  """An activation tensor kept in 8 bits (csmri_act8_save): ``q`` uint8 [pixels, C], ``s`` uint8 [pixels, ceil(C / 32)],
+  ``shape`` and ``dtype`` of what was saved."""
+
+  def __init__(self, q, s, shape, dtype):
+    self.q, self.s, self.shape, self.dtype = q, s, tuple(shape), dtype
+
+
+def _act8_buffers(n, c, device):
+  return (torch.empty(n, c, dtype=torch.uint8, device=device),
+          torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=device))
+
+
+def act8_save(x):
+  """Keep ``x`` (bf16 / fp32) in 8 bits: e4m3 codes, one power-of-two scale per 32 channels of a pixel."""
+  xr, n, c, ps = _pixels(x)
+  q, s = _act8_buffers(n, c, x.device)
+  with _on_device_of(x):
+    lib.call('csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, q.data_ptr(), s.data_ptr(), stream())
+  return Act8(q, s, x.shape, x.dtype)
+
+
+def act8_restore(a, dtype=None):
+  """The values of a kept tensor in its own dtype or ``dtype``."""
+  dtype = a.dtype if dtype is None else dtype
+  out = torch.empty(a.shape, dtype=dtype, device=a.q.device)
+  c = a.shape[-1]
+  with _on_device_of(a.q):
+    lib.call('csmri_act8_restore', a.q.data_ptr(), a.s.data_ptr(), a.q.shape[0], c, dt_of(out), out.data_ptr(), c,
+             stream())
+  return out
+
+
+def act8_wgrad(a, gy, cout=None, cin=None, want_bias=True, dw=None, db=None, accumulate=False):
+  """(dw, db): gradients of a 1 x 1 convolution's weight [cout, cin] and bias [cout] (fp32) from its kept input and the
+  gradient ``gy`` [..., Cout_p] of its output.  ``dw`` / ``db``: written there (added to with ``accumulate``)."""
+  gr, n, cp, ps = _pixels(gy)
+  if tuple(gy.shape[:-1]) != a.shape[:-1]:
+    raise ValueError('csmri_hip: gradient of %s for a kept input of %s' % (tuple(gy.shape), a.shape))
+  cin_p = a.shape[-1]
+  cout, cin = cp if cout is None else cout, cin_p if cin is None else cin
+  dev = gy.device
+  if dw is None:
+    dw, accumulate = torch.empty(cout, cin, dtype=torch.float32, device=dev), False
+    db = torch.empty(cout, dtype=torch.float32, device=dev) if want_bias else None
+  splits = lib.raw('csmri_act8_wgrad_splits')(n, cp, cin_p)
+  nbytes = lib.raw('csmri_act8_wgrad_slab_bytes')(splits, cout, cin)
+  with _on_device_of(gy, a.q, dw, db):
+    slab = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+    lib.call('csmri_act8_wgrad', dt_of(gr), gr.data_ptr(), ps, a.q.data_ptr(), a.s.data_ptr(), n, cp, cin_p, cout, cin,
+             splits, ptr(slab), dw.data_ptr(), ptr(db), int(bool(accumulate)), stream())
+  return dw, db
+
+
+class Mx4(object):
+  """Rows of ``k`` channels in microscaled 4-bit form (csmri_mx4_quantize): ``codes`` uint8 [rows, 64 * ceil(k / 128)],
+  two e2m1 codes a byte, the even channel in the low half; ``scales`` uint8 [rows, 16 * ceil(k / 512)], one E8M0 byte per
+  32 channels.  Padding: code 0, any scale but 255.  ``shape``: of the tensor they stand for."""
+
+  def __init__(self, codes, scales, k, shape=None):
+    cb, sb = lib.raw('csmri_mx4_code_bytes')(k), lib.raw('csmri_mx4_scale_bytes')(k)
+    for t, nb, what in ((codes, cb, 'codes'), (scales, sb, 'scales')):
+      if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != nb or t.shape[0] != codes.shape[0]:
+        raise ValueError('csmri_hip: 4-bit %s of %d channels have to be uint8 [rows, %d], got %s %s' %
+                         (what, k, nb, t.dtype, tuple(t.shape)))
+      if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError('csmri_hip: 4-bit %s have to be contiguous and 16-byte aligned' % what)
+    if k % 8:
+      raise ValueError('csmri_hip: 4-bit rows hold a multiple of 8 channels, got %d' % k)
+    self.codes, self.scales, self.k = codes, scales, k
+    self.shape = (codes.shape[0], k) if shape is None else tuple(shape)
+
+
+def mx4_quantize(x, out=None):
+  """``x`` [..., k] (bf16 / fp32) as 4-bit rows; ``out``: an Mx4 of the same size to overwrite."""
+  xr, n, c, ps = _pixels(x)
+  if out is None:
+    out = Mx4(torch.empty(n, lib.raw('csmri_mx4_code_bytes')(c), dtype=torch.uint8, device=x.device),
+              torch.empty(n, lib.raw('csmri_mx4_scale_bytes')(c), dtype=torch.uint8, device=x.device), c, x.shape)
+  elif out.k != c or out.codes.shape[0] != n:
+    raise ValueError('csmri_hip: 4-bit buffers of %s for a tensor of %s' % (out.shape, tuple(x.shape)))
+  with _on_device_of(x, out.codes, out.scales):
+    lib.call('csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, out.codes.data_ptr(), out.scales.data_ptr(),
+             stream())
+  return out
+
+
+def mx4_dequantize(m, dtype=torch.bfloat16):
+  """The values 4-bit rows stand for (exact in either dtype)."""
+  out = torch.empty(m.shape, dtype=dtype, device=m.codes.device)
+  with _on_device_of(out, m.scales):
+    lib.call('csmri_mx4_dequantize', m.codes.data_ptr(), m.scales.data_ptr(), m.codes.shape[0], m.k, dt_of(out),
+             out.data_ptr(), m.k, stream())
+  return out
+
+
+def mx4_linear(x, w, bias=None, slope=1.0, out_dtype=None):
+  """act(xq wq^T + bias): the 1 x 1 convolution of pixels ``x`` [..., k] (bf16 / fp32, quantised on the way, or an Mx4)
+  with 4-bit weights ``w`` (Mx4 of N rows), act the LeakyReLU of ``slope`` (1: none).  Returns [..., pad8(N)] in
+  ``out_dtype`` (default: of x; bf16 for an Mx4), pad channels zero."""
+  if isinstance(x, Mx4):
+    dev_t, n, k, ps, shape, xdt, xp, sp = x.codes, x.codes.shape[0], x.k, 0, x.shape, MX4, x.codes.data_ptr(), \
+        x.scales.data_ptr()
+    xr = None
+  else:
+    xr, n, k, ps = _pixels(x)
+    dev_t, shape, xdt, xp, sp = x, x.shape, dt_of(xr), xr.data_ptr(), 0
+  if k != w.k:
+    raise ValueError('csmri_hip: %d channels against 4-bit weights of %d' % (k, w.k))
+  cout = w.codes.shape[0]
+  if bias is not None:
+    bias = _vector(bias, cout, 'bias')
+  out_dtype = out_dtype or (torch.bfloat16 if xr is None else x.dtype)
+  y = torch.empty(tuple(shape[:-1]) + (pad8(cout),), dtype=out_dtype, device=dev_t.device)
+  if cout == 0:
+    return y
+  nbytes = lib.raw('csmri_mx4_linear_work_bytes')(xdt, n, k)
+  with _on_device_of(dev_t, w.codes, w.scales, bias):
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev_t.device) if nbytes else None
+    lib.call('csmri_mx4_linear', xdt, xp, ps, sp, n, k, w.codes.data_ptr(), w.scales.data_ptr(), cout, ptr(bias),
+             float(slope), y.data_ptr(), dt_of(y), y.shape[-1], ptr(work), stream())
+  return y
+
+
+class LNSaved(object):
+  """What layer_norm_bwd reads: the input itself or its kept form with the forward's statistics, and the affine
+  parameters as the forward used them."""
+
+  def __init__(self, x, kept, stats, snap, shape, dtype, c_real, eps, slope):
+    self.x, self.kept, self.stats, self.snap = x, kept, stats, snap
+    self.shape, self.dtype, self.c_real, self.eps, self.slope = tuple(shape), dtype, c_real, eps, slope
+
+
+def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
+  """(z, saved): layer norm over the channels of each pixel and LeakyReLU of ``slope`` (1: none).  gamma, beta: fp32
+  [C_real]; channels behind C_real are padding (zero in z).  ``keep8``: ``saved`` holds x in 8 bits, written by the same
+  pass, instead of x."""
+  xr, n, c, ps = _pixels(x)
+  c_real = gamma.shape[0]
+  gamma, beta = _vector(gamma, c_real, 'gamma'), _vector(beta, c_real, 'beta')
+  dev = x.device
+  with _on_device_of(x, gamma, beta):
+    z = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    snap = torch.empty(2, c, dtype=torch.float32, device=dev)
+    q, s = _act8_buffers(n, c, dev) if keep8 else (None, None)
+    stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
+    lib.call('csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
+             beta.data_ptr(), float(eps), float(slope), snap.data_ptr(), ptr(stats), ptr(q), ptr(s), stream())
+  return z, LNSaved(None if keep8 else xr, Act8(q, s, x.shape, x.dtype) if keep8 else None, stats, snap, x.shape,
+                    x.dtype, c_real, float(eps), float(slope))
+
+
+def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None, dbeta=None, accumulate=False):
+  """(gx, dgamma, dbeta) for the gradient ``gz`` of layer_norm's output.  ``z``: that output, needed where the input was
+  kept in 8 bits and the slope is not 1.  ``dgamma`` / ``dbeta``: written there (added to with ``accumulate``)."""
+  if tuple(gz.shape) != saved.shape or gz.dtype != saved.dtype:
+    raise ValueError('csmri_hip: gradient %s %s of a layer norm over %s %s' % (gz.dtype, tuple(gz.shape), saved.dtype, saved.shape))
+  kept = saved.kept
+  if kept is not None and saved.slope != 1.0 and z is None:
+    raise ValueError('csmri_hip: layer_norm_bwd needs z: its input was kept in 8 bits, the sign of the output was not')
+  gr, n, c, gps = _pixels(gz)
+  xr, xps, zr, zps = None, 0, None, 0
+  if kept is None:
+    xr, _, _, xps = _pixels(saved.x)
+  elif saved.slope != 1.0:
+    if tuple(z.shape) != saved.shape or z.dtype != saved.dtype:
+      raise ValueError('csmri_hip: z %s %s of a layer norm over %s %s' % (z.dtype, tuple(z.shape), saved.dtype, saved.shape))
+    zr, _, _, zps = _pixels(z)
+  dev = gz.device
+  with _on_device_of(gz, saved.snap, zr, dgamma, dbeta):
+    gx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if want_x else None
+    partial = None
+    if want_affine:
+      if dgamma is None:
+        dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
+                                     torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
+      partial = torch.empty(lib.raw('csmri_ln_bwd_rows')(n, c), 2, c, dtype=torch.float32, device=dev)
+    lib.call('csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps, ptr(kept.q) if kept else 0,
+             ptr(kept.s) if kept else 0, ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c, saved.c_real,
+             saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
+             ptr(dbeta) if want_affine else 0, int(bool(accumulate)), stream())
+  return gx, dgamma if want_affine else None, dbeta if want_affine else None
+
+
 SPLITK_OVERRIDE = None   # tools/sk_sweep.py only: force the split-K factor of csmri_gconv launches
 GCONV_FLAGS = int(os.environ.get('CSMRI_GCONV_FLAGS', '0'))   # or-ed into csmri_gconv_desc.flags (A/B switches of the conv dispatch: 2 / 16 = gpipe everywhere / nowhere)
 
@@ -458,6 +711,15 @@ def conv_forward(layer, x0, x1=None, use_bias=True, act_slope=1.0, want_stats=Fa
     cin += x1.shape[3]
   assert cin == layer.cin_p, (cin, layer.cin_p)
   assert x0.dtype == layer.dtype
+  if layer.mx4_ok(x1):
+    # 4-bit variant: both operands microscaled, fp32 accumulation, the same epilogue; the BatchNorm statistics are
+    # taken by their own pass
+    if LAUNCH_LOG is not None:
+      LAUNCH_LOG.append(('gconv', 'mx4_linear', 1))
+    with _Timed('mx4_linear', 2.0 * b * h * w * layer.cout * layer.cin):
+      y = mx4_linear(x0, layer._pack_mx4(), layer.bias if use_bias else None, float(act_slope),
+                     out_dtype or layer.dtype)
+    return y, None
   ho, wo = layer.out_hw(h, w)
   odt = out_dtype or layer.dtype
   y = torch.empty(b, ho, wo, layer.cout_p, dtype=odt, device=x0.device)
@@ -587,9 +849,21 @@ def conv_dgrad(layer, gy, in_hw, g_src=None, g_slope=1.0):
 
 
 def conv_wgrad(layer, x0, x1, gy, accumulate=True):
-  """Accumulates dW (and db) into layer.weight.grad / layer.bias.grad (fp32)."""
-  x0 = as_nhwc(x0)
+  """Accumulates dW (and db) into layer.weight.grad / layer.bias.grad (fp32).  ``x0`` / ``x1`` may be kept in 8 bits
+  (Act8): a 1 x 1 layer reads them as they are, the other kernels their restored values."""
   gy = as_nhwc(gy)
+  if isinstance(x0, Act8) and x1 is None and layer.pointwise():
+    dw, db, acc = _grad_targets(layer)
+    if LAUNCH_LOG is not None:
+      LAUNCH_LOG.append(('wgrad', 'act8_wgrad', 1))
+
+    def launch8():
+      with _Timed('act8_wgrad', 2.0 * gy.shape[0] * gy.shape[1] * gy.shape[2] * layer.cout * layer.cin):
+        act8_wgrad(x0, gy, layer.cout, layer.cin, db is not None, dw, db, accumulate and acc)
+
+    return _issue_wgrad(layer, (x0.q, x0.s, gy), launch8)
+  x0, x1 = [act8_restore(t) if isinstance(t, Act8) else t for t in (x0, x1)]
+  x0 = as_nhwc(x0)
   b, h, w, c0 = x0.shape
   _, ho, wo, _ = gy.shape
   wgt = layer.weight
@@ -656,6 +930,11 @@ def conv_wgrad(layer, x0, x1, gy, accumulate=True):
       fq.append((d, slab, wgt.grad, layer.bias.grad if layer.bias is not None else None,
                  torch.cuda.current_stream()))
 
+  _issue_wgrad(layer, (x0, x1, gy), launch)
+
+
+def _issue_wgrad(layer, operands, launch):
+  """Run a weight-gradient launch now, on the side stream, or on the side stream a little later."""
   if _WGRAD['stream'] is None:
     launch()
     return
@@ -666,7 +945,7 @@ def conv_wgrad(layer, x0, x1, gy, accumulate=True):
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
       launch()
-    for t in (x0, x1, gy):
+    for t in operands:
       if t is not None:
         t.record_stream(side)
     _mark_pending(side)
@@ -681,9 +960,9 @@ def conv_wgrad(layer, x0, x1, gy, accumulate=True):
   # whatever is still held back when this backward pass ends is issued then (autograd engine callback): a caller
   # that reads .grad after backward() + synchronize / join_wgrad_stream() sees every launch, as without deferral
   if not _ensure_flush_callback():      # not inside a backward pass (direct call): no deferral
-    _issue_deferred_wgrad((ev, launch, (x0, x1, gy), layer))
+    _issue_deferred_wgrad((ev, launch, operands, layer))
     return
-  q.append((ev, launch, (x0, x1, gy), layer))
+  q.append((ev, launch, operands, layer))
   # (Releasing the held-back launches every N layers as the first successor of the chain's newest node, and two or
   # three weight-gradient streams, were measured slower the more they overlapped with the chain: DESIGN 9.0.)
   while len(q) > WGRAD_DEFER:
@@ -822,6 +1101,27 @@ def _two_grads(ctx, g_a, g_b, dtype):
   return g_a, g_b
 
 
+def _save_conv_inputs(ctx, layer, w_req, x0, x1, *rest):
+  """save_for_backward of a convolution node: its inputs as they are, or in 8 bits (layer.keep8; only the weight
+  gradient reads them), and ``rest``."""
+  ctx.kept = None
+  if layer.keep8 and w_req:
+    kept = [None if t is None else act8_save(t) for t in (x0, x1)]
+    ctx.kept = [None if a is None else (a.shape, a.dtype) for a in kept]
+    ctx.save_for_backward(*([t for a in kept for t in ((None, None) if a is None else (a.q, a.s))] + list(rest)))
+  else:
+    ctx.save_for_backward(x0, x1, *rest)
+
+
+def _saved_conv_inputs(ctx):
+  saved = ctx.saved_tensors
+  kept = getattr(ctx, 'kept', None)
+  if kept is None:
+    return saved
+  x = [None if m is None else Act8(saved[2 * i], saved[2 * i + 1], *m) for i, m in enumerate(kept)]
+  return tuple(x) + tuple(saved[4:])
+
+
 class ConvAct(torch.autograd.Function):
   """pad -> conv -> (+bias) -> LeakyReLU/ReLU, one kernel.  inputs: x0, x1|None,
   weight, bias (the Parameters, so autograd schedules the backward)."""
@@ -832,15 +1132,15 @@ class ConvAct(torch.autograd.Function):
     ctx.layer, ctx.act_slope = layer, act_slope
     ctx.c0 = x0.shape[3]
     ctx.in_hw = (x0.shape[1], x0.shape[2])
-    ctx.save_for_backward(x0, x1, y)
     # captured at forward time: a later pass may toggle layer.train_weights
     ctx.w_req = weight.requires_grad and layer.train_weights
+    _save_conv_inputs(ctx, layer, ctx.w_req, x0, x1, y)
     return y
 
   @staticmethod
   def backward(ctx, gy, gy2=None):
     layer = ctx.layer
-    x0, x1, y = ctx.saved_tensors
+    x0, x1, y = _saved_conv_inputs(ctx)
     gy, gy2 = _two_grads(ctx, gy, gy2, layer.dtype)
     if ctx.act_slope != 1.0:
       g = act_bwd(gy, y, ctx.act_slope, gy2)
@@ -1246,14 +1546,14 @@ class ConvBnAct(torch.autograd.Function):
     ctx.c0 = x0.shape[3]
     ctx.in_hw = (x0.shape[1], x0.shape[2])
     # z is not kept for the BN backward: the activation sign is recomputed from y and `snap`
-    ctx.save_for_backward(x0, x1, y, snap, mean, invstd, dropmask)
     ctx.w_req = weight.requires_grad and layer.train_weights
+    _save_conv_inputs(ctx, layer, ctx.w_req, x0, x1, y, snap, mean, invstd, dropmask)
     return z
 
   @staticmethod
   def backward(ctx, gz, gz2=None):
     layer, bn = ctx.layer, ctx.bn
-    x0, x1, y, snap, mean, invstd, dropmask = ctx.saved_tensors
+    x0, x1, y, snap, mean, invstd, dropmask = _saved_conv_inputs(ctx)
     if not ctx.training:
       raise RuntimeError('backward through eval-mode BatchNorm is not on the training path')
     gz, gz2 = _two_grads(ctx, gz, gz2, layer.dtype)
@@ -1316,6 +1616,64 @@ class ConvBnAct(torch.autograd.Function):
       if GRAD_READY_HOOK is not None and not _wgrad_deferred_mode():
         GRAD_READY_HOOK(layer)
     return gx0, gx1, None, None, None, None, None, None, None, None, None
+
+
+class LayerNormAct(torch.autograd.Function):
+  """layer_norm as an autograd node: z = lrelu(layer norm of x over its channels).  ``keep8``: x is kept in 8 bits.
+  Like the BatchNorm node's, the affine gradients are accumulated into gamma.grad / beta.grad by the kernels."""
+
+  @staticmethod
+  def forward(ctx, x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
+    z, sv = layer_norm(x, gamma, beta, eps, slope, keep8)
+    ctx.gamma, ctx.beta = gamma, beta
+    ctx.affine_req = (gamma.requires_grad, beta.requires_grad)
+    ctx.meta = (sv.shape, sv.dtype, sv.c_real, sv.eps, sv.slope)
+    ctx.keep8 = bool(keep8)
+    if keep8:
+      ctx.save_for_backward(sv.kept.q, sv.kept.s, sv.stats, sv.snap, z if slope != 1.0 else None)
+    else:
+      ctx.save_for_backward(sv.x, sv.snap)
+    return z
+
+  @staticmethod
+  def backward(ctx, gz):
+    z = None
+    if ctx.keep8:
+      q, s, stats, snap, z = ctx.saved_tensors
+      sv = LNSaved(None, Act8(q, s, ctx.meta[0], ctx.meta[1]), stats, snap, *ctx.meta)
+    else:
+      x, snap = ctx.saved_tensors
+      sv = LNSaved(x, None, None, snap, *ctx.meta)
+    if gz.dtype != sv.dtype:
+      gz = gz.to(sv.dtype)
+    want = any(ctx.affine_req)
+    dg = db = None
+    acc = True
+    if want:
+      dg, db, acc = _affine_targets(ctx.gamma, ctx.beta, ctx.affine_req)
+    gx = layer_norm_bwd(gz, sv, z, ctx.needs_input_grad[0], want, dg, db, acc)[0]
+    return gx, None, None, None, None, None
+
+
+def _affine_targets(gamma, beta, req):
+  """(dgamma, dbeta, accumulate): where the kernels write the two gradients, honouring FlatAdam.lazy_zero; a parameter
+  without gradient gets a buffer that is dropped."""
+  fresh = []
+  for p, r in zip((gamma, beta), req):
+    if not r:
+      continue
+    if p.grad is None:
+      p.grad = torch.zeros_like(p)
+    assert p.grad.is_contiguous()
+    p._kernel_grad = True
+    fresh.append(getattr(p, '_grad_fresh', False))
+    if fresh[-1]:
+      p._grad_fresh = False
+  acc = not all(fresh)
+  if acc and any(fresh):                     # one of the two was written since zero_grad(): the other starts from zero
+    [p for p, r in zip((gamma, beta), req) if r][fresh.index(True)].grad.zero_()
+  out = [p.grad if r else torch.zeros_like(p) for p, r in zip((gamma, beta), req)]
+  return out[0], out[1], acc
 
 
 class ConvBnActReplay(torch.autograd.Function):

@@ -43,6 +43,8 @@ extern "C" {
  * dst_dtype of csmri_nchw_to_nhwc (C = 2, Cpad = 8); never a compute dtype. */
 #define CSMRI_BF16_SPLIT 3
 
+#define CSMRI_MX4 4   /* microscaled 4-bit rows (csmri_mx4_quantize): type of an operand of csmri_mx4_linear only */
+
 #define CSMRI_OK 0
 #define CSMRI_E_ARG (-1)
 #define CSMRI_E_UNSUPPORTED (-2)
@@ -639,6 +641,74 @@ int csmri_dropout2d_mask(float* mask, long long n, float p, unsigned long long* 
 int csmri_bucket_pack_bf16(const float* g, long long n, void* send, long long n_padded, void* stream);
 int csmri_bucket_reduce(const void* recv, int world, long long per, void* mine, void* stream);
 int csmri_bucket_unpack_bf16(const void* src, long long n, float* g, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm over the channels of each pixel + LeakyReLU (no counterpart in the reference, whose networks know
+ * nn.BatchNorm2d only: models/unet.py:48-58; a batch of one normalises like any other here).
+ *   m = mean_c x, r = 1 / sqrt(mean_c (x - m)^2 + eps), h = (x - m) r, y = gamma h + beta, z = y > 0 ? y : slope y
+ * npix rows of C channels (a multiple of 8, at most 8192), the first C_real of them real; pad channels of z and dx are
+ * written as zeros.  gamma, beta: [C_real].  affine_snap ([2][C] fp32, 16-byte aligned, optional) receives gamma and beta
+ * as this forward used them.  stats ([2][npix] fp32: m, then r) is optional unless the input is kept.
+ * q8 / s8 (both or neither): x in the 8-bit form of csmri_act8_save, written by the same pass.
+ * z must not be x (E_ARG), and must not overlap it otherwise. */
+int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z, int z_pix_stride, long long npix, int C,
+                 int C_real, const float* gamma, const float* beta, float eps, float slope, float* affine_snap,
+                 float* stats, void* q8, uint8_t* s8, void* stream);
+/* Backward: dy = dz * (y > 0 ? 1 : slope), t = dy gamma, dx = r (t - mean_c t - h mean_c (t h)),
+ * dgamma = sum_p dy h, dbeta = sum_p dy.  The input is either x (m and r are computed again) or q8 / s8 with the
+ * forward's stats; with the kept form and slope != 1, z is needed for the sign of y (optional otherwise).  dx may be
+ * NULL; dgamma and dbeta (both or neither, [C_real], added to where accumulate != 0) need partial:
+ * [csmri_ln_bwd_rows(npix, C)][2][C] fp32, 16-byte aligned.  Fixed summation order. */
+int csmri_ln_bwd_rows(long long npix, int C);
+int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const void* x, int x_pix_stride, const void* q8,
+                 const uint8_t* s8, const float* stats, const void* z, int z_pix_stride, void* dx, int dx_pix_stride,
+                 long long npix, int C, int C_real, const float* affine_snap, float eps, float slope, float* partial,
+                 float* dgamma, float* dbeta, int accumulate, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Activations kept for the backward pass in 8 bits: e4m3fn codes q8 [npix][C] (8-byte aligned, dense) and one E8M0 scale
+ * byte per 32 consecutive channels of a pixel, s8 [npix][ceil(C / 32)] (value 2^(s8 - 127)):
+ *   e = max(floor(log2(max |x| of the block)), -100), s8 = e - 7 + 127, q8 = e4m3_rne(x / 2^(e - 7))
+ * |x / scale| < 256, so nothing saturates.  A block with a NaN or an infinity: s8 = 255, codes NaN, all of it reads NaN.
+ * C % 8 == 0.  csmri_act8_restore writes the values (exact in either dtype; a magnitude within half a step of 2^128
+ * reads as infinity). */
+int csmri_act8_save(int dtype, const void* x, int x_pix_stride, long long npix, int C, void* q8, uint8_t* s8, void* stream);
+int csmri_act8_restore(const void* q8, const uint8_t* s8, long long npix, int C, int dtype, void* out, int out_pix_stride,
+                       void* stream);
+/* Weight gradient of a 1 x 1 stride-1 convolution whose input was kept in 8 bits (csmri_wgrad for that case):
+ *   dw[n][c] (+)= sum_p dy[p][n] xhat[p][c],  db[n] (+)= sum_p dy[p][n]
+ * dw: fp32 [Cout_real][Cin_real]; db: fp32 [Cout_real] or NULL; Cout, Cin: padded channel counts of dy and of the kept
+ * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts.
+ * splits: csmri_act8_wgrad_splits; slab: csmri_act8_wgrad_slab_bytes (NULL when that is 0).  Fixed summation order.
+ * npix == 0 leaves zeros (or what was there, with accumulate). */
+int csmri_act8_wgrad_splits(long long npix, int Cout, int Cin);
+size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real);
+int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride, const void* q8, const uint8_t* s8, long long npix,
+                     int Cout, int Cin, int Cout_real, int Cin_real, int splits, float* slab, float* dw, float* db,
+                     int accumulate, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Microscaled 4-bit rows (OCP MXFP4): e2m1 codes, two a byte with the even channel in the low half, and one E8M0 scale
+ * byte per 32 consecutive channels.  A row of K channels holds csmri_mx4_code_bytes(K) = 64 ceil(K / 128) code bytes and
+ * csmri_mx4_scale_bytes(K) = 16 ceil(K / 512) scale bytes; padding is code 0 and any scale but 255 (the quantiser writes
+ * 2^0).  codes, scales: 16-byte aligned, dense rows.
+ *   e = max(floor(log2(max |x| of the block)), -100), scale 2^(e - 2), code = e2m1_rne(x / scale), saturating at 6
+ * A block with a NaN or an infinity: scale 255, all of it reads NaN.  K % 8 == 0.
+ * ---------------------------------------------------------------------- */
+int csmri_mx4_code_bytes(int K);
+int csmri_mx4_scale_bytes(int K);
+int csmri_mx4_quantize(int dtype, const void* x, int x_pix_stride, long long rows, int K, void* codes, uint8_t* scales,
+                       void* stream);
+int csmri_mx4_dequantize(const void* codes, const uint8_t* scales, long long rows, int K, int dtype, void* out,
+                         int out_pix_stride, void* stream);
+/* 1 x 1 convolution on 4-bit operands: out[p][n] = act(sum_c xq[p][c] wq[n][c] + bias[n]), act(v) = v > 0 ? v : slope v,
+ * n < N; channels N..8 ceil(N / 8) of out are written as zeros (out_pix_stride covers them).  x: fp32 / bf16 pixels,
+ * quantised on the way, or codes (x_dtype CSMRI_MX4, with x_scales; x_pix_stride unused).  w: N rows of K channels.
+ * work: csmri_mx4_linear_work_bytes bytes, 16-byte aligned (NULL when that is 0).  bias may be NULL. */
+size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K);
+int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, const uint8_t* x_scales, long long rows, int K,
+                     const void* w_codes, const uint8_t* w_scales, int N, const float* bias, float slope, void* out,
+                     int out_dtype, int out_pix_stride, void* work, void* stream);
 
 /* misc */
 int csmri_fill_f32(float* p, long long n, float v, void* stream);
