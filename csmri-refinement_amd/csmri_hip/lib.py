@@ -224,14 +224,14 @@ _SIGS = {
                            i32, vp]),
     'csmri_act8_save': (i32, [i32, vp, i32, i64, i32, vp, vp, vp]),
     'csmri_act8_restore': (i32, [vp, vp, i64, i32, i32, vp, i32, vp]),
-    'csmri_act8_wgrad_splits': (i32, [i64, i32, i32]),
+    'csmri_act8_wgrad_splits': (i32, [i32, i64, i32, i32]),
     'csmri_act8_wgrad_slab_bytes': (sz, [i32, i32, i32]),
     'csmri_act8_wgrad': (i32, [i32, vp, i32, vp, vp, i64, i32, i32, i32, i32, i32, vp, vp, vp, i32, vp]),
     'csmri_mx4_code_bytes': (i32, [i32]),
     'csmri_mx4_scale_bytes': (i32, [i32]),
     'csmri_mx4_quantize': (i32, [i32, vp, i32, i64, i32, vp, vp, vp]),
     'csmri_mx4_dequantize': (i32, [vp, vp, i64, i32, i32, vp, i32, vp]),
-    'csmri_mx4_linear_work_bytes': (sz, [i32, i64, i32]),
+    'csmri_mx4_linear_work_bytes': (sz, [i32, i64, i32, i32]),
     'csmri_mx4_linear': (i32, [i32, vp, i32, vp, i64, i32, vp, vp, i32, vp, f32, vp, i32, i32, vp, vp]),
     'csmri_fill_f32': (i32, [vp, i64, f32, vp]),
     'csmri_cast': (i32, [vp, i32, vp, i32, i64, vp]),

@@ -433,37 +433,48 @@ def _pixels(t):
   """(tensor, pixels, channels, pixel stride) of ``t`` [..., C]."""
   _need_gpu(t)
   dt_of(t)
-  c = t.shape[-1] if t.dim() else 0
+  shape = t.shape
+  c = shape[-1] if shape else 0
   if c == 0 or c % 8:
-    raise ValueError('csmri_hip: the channel axis has to be a multiple of 8 (got shape %s)' % (tuple(t.shape),))
+    raise ValueError('csmri_hip: the channel axis has to be a multiple of 8 (got shape %s)' % (tuple(shape),))
   n = t.numel() // c
-  ps, span, ok = c, 0, t.stride(-1) == 1
-  for size, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
-    if size == 1 or n == 0:
-      continue
-    if span == 0:
-      ps, span = st, st * size
-    else:
-      ok, span = ok and st == span, span * size
-  es = t.element_size()
-  if not ok or ps < c or ps * es % 16 or t.data_ptr() % 16:
+  if t.is_contiguous():
+    ps, ok = c, True
+  else:
+    ps, span, ok = c, 0, t.stride(-1) == 1
+    for size, st in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
+      if size == 1 or n == 0:
+        continue
+      if span == 0:
+        ps, span = st, st * size
+      else:
+        ok, span = ok and st == span, span * size
+    ok = ok and ps >= c and ps * t.element_size() % 16 == 0
+  if not ok or t.data_ptr() % 16:
     t, ps = t.contiguous(), c
     if t.data_ptr() % 16:
       t = t.clone()
   return t, n, c, ps
 
 
-def _on_device_of(t, *others):
-  for o in others:
-    if o is not None and o.device != t.device:
+def _launch(t, operands, name, *args):
+  """lib.call on the current stream of ``t``'s device, where all ``operands`` (None: absent) have to live."""
+  dev = t.get_device()
+  for o in operands:
+    if o is not None and o.get_device() != dev:
       raise RuntimeError('csmri_hip: operands on %s and %s' % (t.device, o.device))
-  return torch.cuda.device(t.device)
+  st = torch._C._cuda_getCurrentRawStream(dev)
+  if dev == torch.cuda.current_device():
+    lib.call(name, *args, st)
+  else:
+    with torch.cuda.device(dev):
+      lib.call(name, *args, st)
 
 
 def _vector(t, n, what):
   if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
     raise ValueError('csmri_hip: %s has to be fp32 [%d], got %s %s' % (what, n, t.dtype, tuple(t.shape)))
-  return t.detach().contiguous()
+  return t if t.is_contiguous() else t.contiguous()
 
 
 class Act8(object):
@@ -483,8 +494,7 @@ def act8_save(x):
   """Keep ``x`` (bf16 / fp32) in 8 bits: e4m3 codes, one power-of-two scale per 32 channels of a pixel."""
   xr, n, c, ps = _pixels(x)
   q, s = _act8_buffers(n, c, x.device)
-  with _on_device_of(x):
-    lib.call('csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, q.data_ptr(), s.data_ptr(), stream())
+  _launch(x, (), 'csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, q.data_ptr(), s.data_ptr())
   return Act8(q, s, x.shape, x.dtype)
 
 
@@ -493,9 +503,8 @@ def act8_restore(a, dtype=None):
   dtype = a.dtype if dtype is None else dtype
   out = torch.empty(a.shape, dtype=dtype, device=a.q.device)
   c = a.shape[-1]
-  with _on_device_of(a.q):
-    lib.call('csmri_act8_restore', a.q.data_ptr(), a.s.data_ptr(), a.q.shape[0], c, dt_of(out), out.data_ptr(), c,
-             stream())
+  _launch(out, (a.q, a.s), 'csmri_act8_restore', a.q.data_ptr(), a.s.data_ptr(), a.q.shape[0], c, dt_of(out),
+          out.data_ptr(), c)
   return out
 
 
@@ -511,12 +520,11 @@ def act8_wgrad(a, gy, cout=None, cin=None, want_bias=True, dw=None, db=None, acc
   if dw is None:
     dw, accumulate = torch.empty(cout, cin, dtype=torch.float32, device=dev), False
     db = torch.empty(cout, dtype=torch.float32, device=dev) if want_bias else None
-  splits = lib.raw('csmri_act8_wgrad_splits')(n, cp, cin_p)
+  splits = lib.raw('csmri_act8_wgrad_splits')(dt_of(gr), n, cp, cin_p)
   nbytes = lib.raw('csmri_act8_wgrad_slab_bytes')(splits, cout, cin)
-  with _on_device_of(gy, a.q, dw, db):
-    slab = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-    lib.call('csmri_act8_wgrad', dt_of(gr), gr.data_ptr(), ps, a.q.data_ptr(), a.s.data_ptr(), n, cp, cin_p, cout, cin,
-             splits, ptr(slab), dw.data_ptr(), ptr(db), int(bool(accumulate)), stream())
+  slab = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
+  _launch(gy, (a.q, a.s, dw, db), 'csmri_act8_wgrad', dt_of(gr), gr.data_ptr(), ps, a.q.data_ptr(), a.s.data_ptr(), n, cp,
+          cin_p, cout, cin, splits, ptr(slab), dw.data_ptr(), ptr(db), int(bool(accumulate)))
   return dw, db
 
 
@@ -526,7 +534,7 @@ class Mx4(object):
   32 channels.  Padding: code 0, any scale but 255.  ``shape``: of the tensor they stand for."""
 
   def __init__(self, codes, scales, k, shape=None):
-    cb, sb = lib.raw('csmri_mx4_code_bytes')(k), lib.raw('csmri_mx4_scale_bytes')(k)
+    cb, sb = 64 * ((k + 127) // 128), 16 * ((k + 511) // 512)        # csmri_mx4_code_bytes, csmri_mx4_scale_bytes
     for t, nb, what in ((codes, cb, 'codes'), (scales, sb, 'scales')):
       if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != nb or t.shape[0] != codes.shape[0]:
         raise ValueError('csmri_hip: 4-bit %s of %d channels have to be uint8 [rows, %d], got %s %s' %
@@ -547,18 +555,16 @@ def mx4_quantize(x, out=None):
               torch.empty(n, lib.raw('csmri_mx4_scale_bytes')(c), dtype=torch.uint8, device=x.device), c, x.shape)
   elif out.k != c or out.codes.shape[0] != n:
     raise ValueError('csmri_hip: 4-bit buffers of %s for a tensor of %s' % (out.shape, tuple(x.shape)))
-  with _on_device_of(x, out.codes, out.scales):
-    lib.call('csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, out.codes.data_ptr(), out.scales.data_ptr(),
-             stream())
+  _launch(x, (out.codes, out.scales), 'csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, out.codes.data_ptr(),
+          out.scales.data_ptr())
   return out
 
 
 def mx4_dequantize(m, dtype=torch.bfloat16):
   """The values 4-bit rows stand for (exact in either dtype)."""
   out = torch.empty(m.shape, dtype=dtype, device=m.codes.device)
-  with _on_device_of(out, m.scales):
-    lib.call('csmri_mx4_dequantize', m.codes.data_ptr(), m.scales.data_ptr(), m.codes.shape[0], m.k, dt_of(out),
-             out.data_ptr(), m.k, stream())
+  _launch(out, (m.codes, m.scales), 'csmri_mx4_dequantize', m.codes.data_ptr(), m.scales.data_ptr(), m.codes.shape[0], m.k,
+          dt_of(out), out.data_ptr(), m.k)
   return out
 
 
@@ -582,11 +588,10 @@ def mx4_linear(x, w, bias=None, slope=1.0, out_dtype=None):
   y = torch.empty(tuple(shape[:-1]) + (pad8(cout),), dtype=out_dtype, device=dev_t.device)
   if cout == 0:
     return y
-  nbytes = lib.raw('csmri_mx4_linear_work_bytes')(xdt, n, k)
-  with _on_device_of(dev_t, w.codes, w.scales, bias):
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev_t.device) if nbytes else None
-    lib.call('csmri_mx4_linear', xdt, xp, ps, sp, n, k, w.codes.data_ptr(), w.scales.data_ptr(), cout, ptr(bias),
-             float(slope), y.data_ptr(), dt_of(y), y.shape[-1], ptr(work), stream())
+  nbytes = lib.raw('csmri_mx4_linear_work_bytes')(xdt, n, k, cout)
+  work = torch.empty(nbytes, dtype=torch.uint8, device=dev_t.device) if nbytes else None
+  _launch(dev_t, (w.codes, w.scales, bias), 'csmri_mx4_linear', xdt, xp, ps, sp, n, k, w.codes.data_ptr(),
+          w.scales.data_ptr(), cout, ptr(bias), float(slope), y.data_ptr(), dt_of(y), y.shape[-1], ptr(work))
   return y
 
 
@@ -607,13 +612,12 @@ def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
   c_real = gamma.shape[0]
   gamma, beta = _vector(gamma, c_real, 'gamma'), _vector(beta, c_real, 'beta')
   dev = x.device
-  with _on_device_of(x, gamma, beta):
-    z = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    snap = torch.empty(2, c, dtype=torch.float32, device=dev)
-    q, s = _act8_buffers(n, c, dev) if keep8 else (None, None)
-    stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
-    lib.call('csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
-             beta.data_ptr(), float(eps), float(slope), snap.data_ptr(), ptr(stats), ptr(q), ptr(s), stream())
+  z = torch.empty(x.shape, dtype=x.dtype, device=dev)
+  snap = torch.empty(2, c, dtype=torch.float32, device=dev)
+  q, s = _act8_buffers(n, c, dev) if keep8 else (None, None)
+  stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
+  _launch(x, (gamma, beta), 'csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
+          beta.data_ptr(), float(eps), float(slope), snap.data_ptr(), ptr(stats), ptr(q), ptr(s))
   return z, LNSaved(None if keep8 else xr, Act8(q, s, x.shape, x.dtype) if keep8 else None, stats, snap, x.shape,
                     x.dtype, c_real, float(eps), float(slope))
 
@@ -635,18 +639,17 @@ def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None
       raise ValueError('csmri_hip: z %s %s of a layer norm over %s %s' % (z.dtype, tuple(z.shape), saved.dtype, saved.shape))
     zr, _, _, zps = _pixels(z)
   dev = gz.device
-  with _on_device_of(gz, saved.snap, zr, dgamma, dbeta):
-    gx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if want_x else None
-    partial = None
-    if want_affine:
-      if dgamma is None:
-        dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
-                                     torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
-      partial = torch.empty(lib.raw('csmri_ln_bwd_rows')(n, c), 2, c, dtype=torch.float32, device=dev)
-    lib.call('csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps, ptr(kept.q) if kept else 0,
-             ptr(kept.s) if kept else 0, ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c, saved.c_real,
-             saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
-             ptr(dbeta) if want_affine else 0, int(bool(accumulate)), stream())
+  gx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if want_x else None
+  partial = None
+  if want_affine:
+    if dgamma is None:
+      dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
+                                   torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
+    partial = torch.empty(lib.raw('csmri_ln_bwd_rows')(n, c), 2, saved.c_real, dtype=torch.float32, device=dev)
+  _launch(gz, (saved.snap, xr, zr, dgamma, dbeta), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps,
+          ptr(kept.q) if kept else 0, ptr(kept.s) if kept else 0, ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c,
+          saved.c_real, saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
+          ptr(dbeta) if want_affine else 0, int(bool(accumulate)))
   return gx, dgamma if want_affine else None, dbeta if want_affine else None
 
 

@@ -101,16 +101,16 @@ extern "C" int csmri_act8_restore(const void* q8, const uint8_t* s8, long long n
 }
 
 // ---- column sums of partial rows ------------------------------------------------------------------------------------
-// 16 columns x 64 row lanes per workgroup: the few columns of a narrow layer still spread their rows over 64 loads in
-// flight, and a row's 64 bytes are one sector.
-__global__ __launch_bounds__(1024) void colsum_rows_kernel(const float* __restrict__ partial, int rows,
-                                                           long long row_stride, long long cols,
-                                                           float* __restrict__ out, int accumulate) {
+// Columns [0, na) go to oa, [na, na + nb) to ob.  Many rows of few columns: 16 columns x 64 row lanes per workgroup, so
+// that the loads of a column spread over the lanes, and a row's 64 bytes are one sector.
+__global__ __launch_bounds__(1024) void colsum_rows_kernel(const float* __restrict__ partial, int rows, long long row_stride,
+                                                           long long na, float* __restrict__ oa, long long nb,
+                                                           float* __restrict__ ob, int accumulate) {
   __shared__ float red[64][17];
   const int cl = threadIdx.x & 15, rl = threadIdx.x >> 4;
   const long long col = (long long)blockIdx.x * 16 + cl;
   float a = 0.f;
-  if (col < cols) {
+  if (col < na + nb) {
     int r = rl;
     for (; r + 192 < rows; r += 256) {
       float t[4];
@@ -127,13 +127,40 @@ __global__ __launch_bounds__(1024) void colsum_rows_kernel(const float* __restri
     if (rl < o) red[rl][cl] += red[rl + o][cl];
     __syncthreads();
   }
-  if (rl == 0 && col < cols) out[col] = (accumulate ? out[col] : 0.f) + red[0][cl];
+  if (rl == 0 && col < na + nb) {
+    float* o = col < na ? oa + col : ob + (col - na);
+    *o = (accumulate ? *o : 0.f) + red[0][cl];
+  }
 }
-int micro_colsum(const float* partial, int rows, long long row_stride, long long cols, float* out, int accumulate,
-                 hipStream_t st) {
-  const long long grid = (cols + 15) / 16;
-  hipLaunchKernelGGL(colsum_rows_kernel, dim3((unsigned)grid), dim3(1024), 0, st, partial, rows, row_stride, cols, out,
-                     accumulate);
+// Few rows of many columns: a thread per column, its rows' loads in batches of four.
+__global__ __launch_bounds__(256) void colsum_cols_kernel(const float* __restrict__ partial, int rows, long long row_stride,
+                                                          long long na, float* __restrict__ oa, long long nb,
+                                                          float* __restrict__ ob, int accumulate) {
+  for (long long col = (long long)blockIdx.x * 256 + threadIdx.x; col < na + nb; col += (long long)gridDim.x * 256) {
+    float a = 0.f;
+    int r = 0;
+    for (; r + 4 <= rows; r += 4) {
+      float t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[u] = partial[(long long)(r + u) * row_stride + col];
+      a += (t[0] + t[1]) + (t[2] + t[3]);
+    }
+    for (; r < rows; ++r) a += partial[(long long)r * row_stride + col];
+    float* o = col < na ? oa + col : ob + (col - na);
+    *o = (accumulate ? *o : 0.f) + a;
+  }
+}
+int micro_colsum2(const float* partial, int rows, long long row_stride, long long na, float* oa, long long nb, float* ob,
+                  int accumulate, hipStream_t st) {
+  const long long cols = na + nb;
+  if (rows > 16 && cols <= 65536) {
+    hipLaunchKernelGGL(colsum_rows_kernel, dim3((unsigned)((cols + 15) / 16)), dim3(1024), 0, st, partial, rows, row_stride,
+                       na, oa, nb, ob, accumulate);
+  } else {
+    const long long want = (cols + 255) / 256;
+    hipLaunchKernelGGL(colsum_cols_kernel, dim3((unsigned)(want < 8192 ? want : 8192)), dim3(256), 0, st, partial, rows,
+                       row_stride, na, oa, nb, ob, accumulate);
+  }
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }
@@ -172,116 +199,198 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
   }
 }
 
-// BT x BT tile (BT output channels x BT input channels), KP pixels per step, 4 waves in 2 x 2
-template <int DT, int BT>
-__global__ __launch_bounds__(256) void act8_wgrad_kernel(const A8WParams p) {
-  constexpr int KP = 32, CPR = BT / 8, PL = DT == CSMRI_F32 ? 3 : 1;
-  constexpr int IMG = KP * BT * 2, NCH = KP * CPR / 256;        // chunks of 8 channels per thread and image
-  constexpr int F = BT / 32;
-  __shared__ __attribute__((aligned(16))) char smem[IMG * (PL + 1)];
-  char* xi = smem + IMG * PL;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wn = wid >> 1, wc = wid & 1;
+__device__ __attribute__((aligned(16))) char a8_zero_page[16];
+typedef __attribute__((address_space(1))) const void* a8g_t;
+typedef __attribute__((address_space(3))) void* a8l_t;
+
+// A workgroup of WN x WC waves takes a tile of 16 FN WN output x 16 FC WC input channels over a range of pixels, KP at a
+// time.  A bf16 dY goes to LDS by LDS-DMA into a ring of three stages; the kept input passes through registers, where
+// its codes become bf16, into one of two; what is loaded during step k is waited for in step k + 1, needed in step k + 2.
+template <int DT, int FN, int FC, int WN, int WC>
+__global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WParams p) {
+  constexpr int NW = WN * WC, NT = 64 * NW, BN = 16 * FN * WN, BC = 16 * FC * WC, KP = 32, CN = BN / 8, CC = BC / 8;
+  constexpr bool SPLIT = DT == CSMRI_F32;
+  constexpr int PL = SPLIT ? 3 : 1, YST = SPLIT ? 2 : 3;         // planes of dY, stages of dY
+  constexpr int YIMG = KP * BN * 2, XIMG = KP * BC * 2;
+  constexpr int NY = KP * CN / NT, NX = KP * CC / NT;            // 16-byte chunks (eight channels) a thread and stage
+  static_assert(KP * CN % NT == 0 && KP * CC % NT == 0, "whole chunks per thread");
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* ximg = smem + YST * PL * YIMG;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid / WC, wc = wid % WC;
   const int tiles = p.ntiles * p.ctiles;
   const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
   const int nt = tile / p.ctiles, ct = tile - nt * p.ctiles;
-  const int n0 = nt * BT, c0 = ct * BT;
+  const int n0 = nt * BN, c0 = ct * BC;
   const long long pb = split * p.chunk, pe = pb + p.chunk < p.npix ? pb + p.chunk : p.npix;
   const int sblocks = (p.Cin + MICRO_BLOCK - 1) / MICRO_BLOCK;
+  const int steps = pe > pb ? (int)((pe - pb + KP - 1) / KP) : 0;
 
-  f32x4_t acc[F][F], accb[F];
+  f32x4_t acc[FN][FC], accb[FN];
 #pragma unroll
-  for (int i = 0; i < F; ++i) {
+  for (int i = 0; i < FN; ++i) {
     accb[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < F; ++j) acc[i][j] = accb[i];
+    for (int j = 0; j < FC; ++j) acc[i][j] = accb[i];
   }
   const bool want_b = p.db && ct == 0 && wc == 0;
   const bf16x8_t ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
-  // fragment addresses: a 16-lane group reads 4 pixel rows x 16 channels
-  const int g = lane >> 4, tr = (lane & 15) >> 2, tc = lane & 3;
 
-  for (long long k0 = pb; k0 < pe; k0 += KP) {
-    raw8<DT> dv[NCH]; u32x2_t xv[NCH]; unsigned char sv[NCH];
+  // chunk j of a thread: slot (row, place) of the image in thread order; the swizzle puts another chunk of the row there
+  const char* yp[NY]; int yrow[NY]; bool yok[NY];
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int id = j * 256 + tid, row = id / CPR, ch = id % CPR;
-      const long long pix = k0 + row;
-      const bool ok = pix < pe;
-      dv[j] = raw8<DT>{}; xv[j] = (u32x2_t){0, 0}; sv[j] = 0;
-      if (ok && n0 + ch * 8 < p.Cout) dv[j] = ldraw8<DT>(p.dy, pix * p.dyps + n0 + ch * 8);
-      if (ok && c0 + ch * 8 < p.Cin) {
-        xv[j] = *(const u32x2_t*)(p.q + pix * p.Cin + c0 + ch * 8);
-        sv[j] = p.s[pix * sblocks + ((c0 + ch * 8) >> 5)];
-      }
-    }
-    __syncthreads();
+  for (int j = 0; j < NY; ++j) {
+    const int id = (j * NW + wid) * 64 + lane, row = id / CN, place = id % CN;
+    const int ch = (img_off<CN>(row, place) >> 4) % CN;
+    yrow[j] = row; yok[j] = n0 + ch * 8 < p.Cout;
+    yp[j] = p.dy + ((pb + row) * p.dyps + n0 + ch * 8) * (SPLIT ? 4 : 2);
+  }
+  const unsigned char* xp[NX]; const unsigned char* sp[NX]; int xrow[NX]; bool xok[NX]; int xoff[NX];
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) {
-      const int id = j * 256 + tid, row = id / CPR, ch = id % CPR, off = img_off<CPR>(row, ch);
-      if constexpr (DT == CSMRI_F32) {
-        float f[8]; u32x4_t o[3];
-        cvt8<DT>(dv[j], f);
-        split3(f, o);
+  for (int j = 0; j < NX; ++j) {
+    const int id = j * NT + tid, row = id / CC, ch = id % CC;
+    xrow[j] = row; xok[j] = c0 + ch * 8 < p.Cin;
+    xp[j] = p.q + (pb + row) * p.Cin + c0 + ch * 8;
+    sp[j] = p.s + (pb + row) * sblocks + ((c0 + ch * 8) >> 5);
+    xoff[j] = img_off<CC>(row, ch);
+  }
+  const long long ystep = (long long)KP * p.dyps * (SPLIT ? 4 : 2), xstep = (long long)KP * p.Cin, sstep = (long long)KP * sblocks;
+  raw8<DT> yv[SPLIT ? NY : 1]; u32x2_t xv[NX]; unsigned sv[NX];
+  auto fetch = [&](int k) {                       // loads of step k; pixels behind the range and channels behind the end: zeros
+    const int left = (int)(pe - pb - (long long)k * KP < KP ? pe - pb - (long long)k * KP : KP);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) *(u32x4_t*)(smem + i * IMG + off) = o[i];
+    for (int j = 0; j < NY; ++j) {
+      const char* src = yp[j] + k * ystep;
+      const bool ok = yok[j] && yrow[j] < left;
+      if constexpr (SPLIT) {
+        yv[j] = raw8<DT>{};
+        if (ok) yv[j] = ldraw8<DT>(src, 0);
       } else {
-        *(u32x4_t*)(smem + off) = dv[j].a;
+        __builtin_amdgcn_global_load_lds((a8g_t)(ok ? src : a8_zero_page), (a8l_t)(smem + (k % 3) * YIMG + (j * NW + wid) * 1024), 16, 0, 0);
       }
-      float v[8];
-      micro_unpack8(xv[j], micro_scale(sv[j]), v);
-      st8<CSMRI_BF16>(xi + off, 0, v);
     }
-    __syncthreads();
-    bf16x8_t xf[F];
-    // pixel rows 8 g + (0..3) and 8 g + (4..7) of the step, 16 channels each
-    const int lo = 8 * g + tr, hi = lo + 4;
 #pragma unroll
-    for (int j = 0; j < F; ++j) {
-      const int ch = (wc * (BT / 2) + j * 16) / 8 + (tc >> 1), in = (tc & 1) * 8;
-      xf[j] = tr_frag(xi, img_off<CPR>(lo, ch) + in, img_off<CPR>(hi, ch) + in);
+    for (int j = 0; j < NX; ++j) {
+      const bool ok = xok[j] && xrow[j] < left;
+      xv[j] = *(const u32x2_t*)(ok ? (const char*)xp[j] + k * xstep : a8_zero_page);
+      sv[j] = *(const unsigned char*)(ok ? (const char*)sp[j] + k * sstep : a8_zero_page);
     }
+  };
+  auto place = [&](int k) {                       // what went through registers -> LDS
+    if constexpr (SPLIT) {
+#pragma unroll
+      for (int j = 0; j < NY; ++j) {
+        float f[8]; u32x4_t o[3];
+        cvt8<DT>(yv[j], f);
+        split3(f, o);
+        char* dst = smem + (k & 1) * PL * YIMG + (j * NW + wid) * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) *(u32x4_t*)(dst + i * YIMG) = o[i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NX; ++j) {
+      const float s = __uint_as_float(sv[j] << 23);
+      u32x4_t o;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        o[2 * q] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, false));
+        o[2 * q + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, true));
+      }
+      *(u32x4_t*)(ximg + (k & 1) * XIMG + xoff[j]) = o;
+    }
+  };
+  auto barrier = [&]() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // fragments: a 16-lane group reads 4 pixel rows x 16 channels; rows 8 g + (0..3) and 8 g + (4..7) of the step
+  const int g = lane >> 4, tr = (lane & 15) >> 2, tc = lane & 3, lo = 8 * g + tr, hi = lo + 4;
+  const int yc = wn * FN * 2 + (tc >> 1), xc = wc * FC * 2 + (tc >> 1), in = (tc & 1) * 8;
+  auto multiply = [&](int k) {
+    const char* yi = smem + (SPLIT ? (k & 1) * PL : k % 3) * YIMG;
+    const char* xi = ximg + (k & 1) * XIMG;
+    bf16x8_t xf[FC];
+#pragma unroll
+    for (int j = 0; j < FC; ++j) xf[j] = tr_frag(xi, img_off<CC>(lo, xc + 2 * j) + in, img_off<CC>(hi, xc + 2 * j) + in);
 #pragma unroll
     for (int pl = 0; pl < PL; ++pl)
 #pragma unroll
-      for (int i = 0; i < F; ++i) {
-        const int ch = (wn * (BT / 2) + i * 16) / 8 + (tc >> 1), in = (tc & 1) * 8;
-        const bf16x8_t yf = tr_frag(smem + pl * IMG, img_off<CPR>(lo, ch) + in, img_off<CPR>(hi, ch) + in);
+      for (int i = 0; i < FN; ++i) {
+        const bf16x8_t yf = tr_frag(yi + pl * YIMG, img_off<CN>(lo, yc + 2 * i) + in, img_off<CN>(hi, yc + 2 * i) + in);
 #pragma unroll
-        for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, xf[j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, xf[j], acc[i][j], 0, 0, 0);
         if (want_b) accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, ones, accb[i], 0, 0, 0);
       }
+  };
+  if (steps > 0) {
+    fetch(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    place(0);
+    fetch(1);
+    for (int k = 0; k < steps; ++k) {
+      barrier();                                  // stage k is there for everyone; everyone has read stage k - 1
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      place(k + 1);
+      fetch(k + 2);
+      multiply(k);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   // lane l holds rows n = 4 g + r, column c = l & 15 of each fragment
   const long long len = (long long)p.Cout_real * p.Cin_real;
   float* dw = p.splits > 1 ? p.slab + split * (len + p.Cout_real) : p.dw;
   float* db = p.splits > 1 ? dw + len : p.db;
   const bool add = p.splits == 1 && p.accumulate;
+  const int cb = c0 + wc * FC * 16 + (lane & 15);
 #pragma unroll
-  for (int i = 0; i < F; ++i)
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int n = n0 + wn * (BT / 2) + i * 16 + 4 * g + r;
+      const int n = n0 + (wn * FN + i) * 16 + 4 * g + r;
       if (n >= p.Cout_real) continue;
+      float* o = dw + (long long)n * p.Cin_real + cb;
+      float old[FC];
 #pragma unroll
-      for (int j = 0; j < F; ++j) {
-        const int c = c0 + wc * (BT / 2) + j * 16 + (lane & 15);
-        if (c >= p.Cin_real) continue;
-        float* o = dw + (long long)n * p.Cin_real + c;
-        *o = acc[i][j][r] + (add ? *o : 0.f);
-      }
+      for (int j = 0; j < FC; ++j) old[j] = add && cb + 16 * j < p.Cin_real ? o[16 * j] : 0.f;
+#pragma unroll
+      for (int j = 0; j < FC; ++j)
+        if (cb + 16 * j < p.Cin_real) o[16 * j] = acc[i][j][r] + old[j];
       if (want_b && (lane & 15) == 0) db[n] = accb[i][r] + (add ? db[n] : 0.f);
     }
 }
 
-static int a8w_tile(int Cout, int Cin) { return Cout <= 64 || Cin <= 64 ? 64 : 128; }
-extern "C" int csmri_act8_wgrad_splits(long long npix, int Cout, int Cin) {
+// tile: 64 or 128 a side by the channel counts, 256 x 256 where that still fills half the chip's CUs with one split each
+struct A8WTile { int bn, bc; };
+static A8WTile a8w_tile(int dtype, long long npix, int Cout, int Cin) {
+  if (dtype == CSMRI_BF16 && (long long)cdiv(Cout, 256) * cdiv(Cin, 256) * (npix / 2048) >= 128 && Cout > 128 && Cin > 128)
+    return {256, 256};
+  return {Cout <= 64 ? 64 : 128, Cin <= 64 ? 64 : 128};
+}
+extern "C" int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin) {
   if (npix <= 0 || Cout <= 0 || Cin <= 0) return 1;
-  const int bt = a8w_tile(Cout, Cin);
-  const long long tiles = (long long)cdiv(Cout, bt) * cdiv(Cin, bt);
-  long long s = 512 / tiles;                                  // two workgroups a CU
-  const long long most = npix / 256;                          // at least eight steps each
+  const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
+  const long long tiles = (long long)cdiv(Cout, t.bn) * cdiv(Cin, t.bc);
+  // one workgroup of the large tile a CU, two of the others; at least sixteen steps each
+  long long s = (t.bn == 256 ? 256 : 512) / tiles;
+  const long long most = npix / 512;
   if (s > most) s = most;
   return s < 1 ? 1 : (int)s;
+}
+template <int DT, int FN, int FC, int WN, int WC> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
+  constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = 32 * 2 * (BN * (DT == CSMRI_F32 ? 6 : 3) + BC * 2);
+  auto kern = act8_wgrad_kernel<DT, FN, FC, WN, WC>;
+  CSMRI_SET_MAX_LDS(kern, LDS);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WN * WC), LDS, st, p);
+  CSMRI_LAUNCH_CHECK();
+  return CSMRI_OK;
+}
+template <int DT> static int a8w_dispatch(const A8WTile& t, const A8WParams& p, unsigned grid, hipStream_t st) {
+  if constexpr (DT == CSMRI_BF16) if (t.bn == 256) return a8w_launch<DT, 8, 4, 2, 4>(p, grid, st);
+  if (t.bn == 128) return t.bc == 128 ? a8w_launch<DT, 4, 4, 2, 2>(p, grid, st) : a8w_launch<DT, 4, 2, 2, 2>(p, grid, st);
+  return t.bc == 128 ? a8w_launch<DT, 2, 4, 2, 2>(p, grid, st) : a8w_launch<DT, 2, 2, 2, 2>(p, grid, st);
 }
 extern "C" size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real) {
   return splits > 1 ? (size_t)splits * ((size_t)Cout_real * Cin_real + Cout_real) * sizeof(float) : 0;
@@ -301,21 +410,15 @@ extern "C" int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride,
   p.q = (const unsigned char*)q8; p.s = (const unsigned char*)s8;
   p.npix = npix;
   p.Cout = Cout; p.Cin = Cin; p.Cout_real = Cout_real; p.Cin_real = Cin_real;
-  const int bt = a8w_tile(Cout, Cin);
-  p.ntiles = cdiv(Cout, bt); p.ctiles = cdiv(Cin, bt);
+  const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
+  p.ntiles = cdiv(Cout, t.bn); p.ctiles = cdiv(Cin, t.bc);
   p.splits = splits; p.slab = slab; p.dw = dw; p.db = db; p.accumulate = accumulate;
   p.chunk = ((npix + splits - 1) / splits + 31) / 32 * 32;
   const long long grid = (long long)p.ntiles * p.ctiles * splits;
   if (grid > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
-  auto kern = dy_dtype == CSMRI_F32 ? (bt == 64 ? act8_wgrad_kernel<CSMRI_F32, 64> : act8_wgrad_kernel<CSMRI_F32, 128>)
-                                    : (bt == 64 ? act8_wgrad_kernel<CSMRI_BF16, 64> : act8_wgrad_kernel<CSMRI_BF16, 128>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), 0, st, p);
-  CSMRI_LAUNCH_CHECK();
-  if (splits > 1) {
-    const long long len = (long long)Cout_real * Cin_real;
-    int rc = micro_colsum(slab, splits, len + Cout_real, len, dw, accumulate, st);
-    if (rc == CSMRI_OK && db) rc = micro_colsum(slab + len, splits, len + Cout_real, Cout_real, db, accumulate, st);
-    return rc;
-  }
-  return CSMRI_OK;
+  const int rc = dy_dtype == CSMRI_F32 ? a8w_dispatch<CSMRI_F32>(t, p, (unsigned)grid, st)
+                                       : a8w_dispatch<CSMRI_BF16>(t, p, (unsigned)grid, st);
+  if (rc != CSMRI_OK || splits == 1) return rc;
+  const long long len = (long long)Cout_real * Cin_real;
+  return micro_colsum2(slab, splits, len + Cout_real, len, dw, db ? Cout_real : 0, db, accumulate, st);
 }

@@ -25,7 +25,7 @@ struct LNParams {
   const float* gamma; const float* beta; float* snap;  // forward: parameters and their snapshot
   const float* stats_in; float* stats_out;             // [2][rows] mean, 1 / std
   float eps, slope;
-  float* partial;                                      // backward: [gridDim.x][2][C], NULL when neither is wanted
+  float* partial;                                      // backward: [gridDim.x][2][C_real], NULL when neither is wanted
 };
 
 // sum over the lanes of a row
@@ -261,11 +261,13 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
     }
   }
   if (!p.partial) return;
-  float* prow = p.partial + (long long)blockIdx.x * 2 * p.C;
+  float* prow = p.partial + (long long)blockIdx.x * 2 * p.C_real;      // dense: both sums are one launch
   if constexpr (WG) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (c[j] < p.C) { st8<CSMRI_F32>(prow, c[j], dg[j]); st8<CSMRI_F32>(prow, p.C + c[j], db[j]); }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k < nv[j]) { prow[c[j] + k] = dg[j][k]; prow[p.C_real + c[j] + k] = db[j][k]; }
   } else {
     // groups of a wave first, then the four waves in order
 #pragma unroll
@@ -287,7 +289,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
       }
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < 2 * p.C; i += 256) prow[i] = part[i < p.C ? i : span + i - p.C];
+    for (int i = threadIdx.x; i < 2 * p.C_real; i += 256) prow[i] = part[i < p.C_real ? i : span + i - p.C_real];
   }
 }
 
@@ -395,7 +397,7 @@ extern "C" int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const 
   CSMRI_CHECK_ARG(!dx || (dx != dz && dx != x && dx != z));
   if (!ln_aligned(dz, dz_pix_stride, dtype) || (x && !ln_aligned(x, x_pix_stride, dtype)) ||
       (z && !ln_aligned(z, z_pix_stride, dtype)) || (dx && !ln_aligned(dx, dx_pix_stride, dtype)) ||
-      ((uintptr_t)q8 & 7) || ((uintptr_t)partial & 15) || ((uintptr_t)affine_snap & 15)) return CSMRI_E_ALIGN;
+      ((uintptr_t)q8 & 7) || ((uintptr_t)affine_snap & 15)) return CSMRI_E_ALIGN;
   LNParams p = {};
   p.x = x; p.xps = x_pix_stride;
   p.q = (const unsigned char*)q8; p.s = s8; p.stats_in = stats;
@@ -412,7 +414,5 @@ extern "C" int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const 
   if (dtype == CSMRI_F32) rc = q8 ? ln_bwd_launch<CSMRI_F32, true>(p, s, blocks, st) : ln_bwd_launch<CSMRI_F32, false>(p, s, blocks, st);
   else rc = q8 ? ln_bwd_launch<CSMRI_BF16, true>(p, s, blocks, st) : ln_bwd_launch<CSMRI_BF16, false>(p, s, blocks, st);
   if (rc != CSMRI_OK || !dgamma) return rc;
-  rc = micro_colsum(partial, blocks, 2LL * C, C_real, dgamma, accumulate, st);
-  if (rc != CSMRI_OK) return rc;
-  return micro_colsum(partial + C, blocks, 2LL * C, C_real, dbeta, accumulate, st);
+  return micro_colsum2(partial, blocks, 2LL * C_real, C_real, dgamma, C_real, dbeta, accumulate, st);
 }

@@ -120,7 +120,7 @@ static inline dim3 row_walk_grid(long long rows, int slots, int unroll) {
   return dim3((unsigned)(gx < 1 ? 1 : gx), (unsigned)gy);
 }
 
-// out[col] (+)= sum over rows of partial[row][col], fixed order; gridDim.x = ceil(cols / 16), 1024 threads.
-// Defined in act8.hip; the weight gradient's slabs and the layer norm's affine partials end in it.
-int micro_colsum(const float* partial, int rows, long long row_stride, long long cols, float* out, int accumulate,
-                 hipStream_t st);
+// oa[col] (+)= sum over rows of partial[row][col] for col < na, ob[col] likewise for the nb columns behind them, in a fixed
+// order (act8.hip; the weight gradient's slabs and the layer norm's affine partials end in it)
+int micro_colsum2(const float* partial, int rows, long long row_stride, long long na, float* oa, long long nb, float* ob,
+                  int accumulate, hipStream_t st);

@@ -149,6 +149,7 @@ struct MxParams {
   void* out; int out_dt, ops;
   long long M; int N, Npad, K, ksteps, cb, sb;   // ksteps: 128-channel steps; cb, sb: code and scale bytes of a row
   int mtiles, ntiles;
+  int splits, schunk; float* slab;               // splits of the channels, schunk steps each; [splits][M][Npad] partial sums
 };
 
 // four consecutive outputs n..n+3 of row m
@@ -176,36 +177,56 @@ __global__ __launch_bounds__(512) void mx4_skinny_kernel(const MxParams p) {
   f32x4_t acc[MF];
 #pragma unroll
   for (int f = 0; f < MF; ++f) acc[f] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  for (int k = wid; k < p.ksteps; k += 8) {
-    const i32x8_t wv = mx4_operand(*(const u32x4_t*)(wrow + k * 64));
-    const int wsc = wsrow[k * 4];
+  constexpr int U = MF == 1 ? 4 : 2;               // steps whose loads are in flight together
+  for (int kb = wid; kb < p.ksteps; kb += 8 * U) {
+    u32x4_t wc[U], xc[U][MF]; int wsc[U], xsc[U][MF];
+    raw8<QX < 0 ? CSMRI_BF16 : QX> raw[QX < 0 ? 1 : U][MF][4];
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
-      const long long m = f * 16 + r16;
-      u32x4_t xc = {0, 0, 0, 0}; int xsc = 127;
-      if constexpr (QX < 0) {
-        if (m < p.M) { xc = *(const u32x4_t*)(p.xq + m * p.cb + k * 64 + g * 16); xsc = p.xs[m * p.sb + k * 4 + g]; }
-      } else {
-        const int c = k * 128 + g * 32;
-        float v[4][8];
-        unsigned amax = 0;
+    for (int u = 0; u < U; ++u) {
+      // a step behind the end: code 0, scale 1
+      const int k = kb + 8 * u;
+      const bool in = k < p.ksteps;
+      wc[u] = (u32x4_t){0, 0, 0, 0}; wsc[u] = 127;
+      if (in) { wc[u] = *(const u32x4_t*)(wrow + k * 64); wsc[u] = wsrow[k * 4]; }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          raw8<QX> raw = raw8<QX>{};
-          if (m < p.M && c + i * 8 < p.K) raw = ldraw8<QX>(p.x, m * p.xps + c + i * 8);
-          cvt8<QX>(raw, v[i]);
+      for (int f = 0; f < MF; ++f) {
+        const long long m = f * 16 + r16;
+        xc[u][f] = (u32x4_t){0, 0, 0, 0}; xsc[u][f] = 127;
+        if constexpr (QX < 0) {
+          if (in && m < p.M) { xc[u][f] = *(const u32x4_t*)(p.xq + m * p.cb + k * 64 + g * 16); xsc[u][f] = p.xs[m * p.sb + k * 4 + g]; }
+        } else {
+          const int c = k * 128 + g * 32;
 #pragma unroll
-          for (int q = 0; q < 8; ++q) { const unsigned a = abs_bits(v[i][q]); amax = a > amax ? a : amax; }
+          for (int i = 0; i < 4; ++i) {
+            raw[u][f][i] = {};
+            if (m < p.M && c + i * 8 < p.K) raw[u][f][i] = ldraw8<QX>(p.x, m * p.xps + c + i * 8);
+          }
         }
-        const int e = micro_exp(amax) - 2;
-        const bool fin = micro_finite(amax);
-        const float s = exp2i(fin ? e : 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) xc[i] = mx4_pack8(v[i], s);
-        xsc = fin ? e + 127 : MICRO_NAN;
       }
-      acc[f] = mx4_mfma(wv, wsc, mx4_operand(xc), xsc, acc[f]);
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int f = 0; f < MF; ++f) {
+        if constexpr (QX >= 0) {
+          float v[4][8];
+          unsigned amax = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            cvt8<QX>(raw[u][f][i], v[i]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) { const unsigned a = abs_bits(v[i][q]); amax = a > amax ? a : amax; }
+          }
+          const int e = micro_exp(amax) - 2;
+          const bool fin = micro_finite(amax);
+          const float s = exp2i(fin ? e : 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) xc[u][f][i] = mx4_pack8(v[i], s);
+          xsc[u][f] = fin ? e + 127 : MICRO_NAN;
+        }
+        acc[f] = mx4_mfma(mx4_operand(wc[u]), wsc[u], mx4_operand(xc[u][f]), xsc[u][f], acc[f]);
+      }
   }
   // lane holds outputs n = n0 + 4 g + r of row m = 16 f + r16
 #pragma unroll
@@ -225,74 +246,243 @@ __global__ __launch_bounds__(512) void mx4_skinny_kernel(const MxParams p) {
   }
 }
 
-// 128 rows x 128 outputs per workgroup, 4 waves of 64 x 64, both operands through LDS, 128 channels a step
-__device__ __forceinline__ int mx_off(int row, int chunk) { return row * 64 + ((chunk ^ ((4 - ((row >> 2) & 3)) & 3)) << 4); }
-__global__ __launch_bounds__(256) void mx4_gemm_kernel(const MxParams p) {
-  constexpr int BM = 128, BN = 128, IMG = 128 * 64;
-  __shared__ __attribute__((aligned(16))) char smem[2 * IMG];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wm = wid >> 1, wn = wid & 1, r16 = lane & 15, g = lane >> 4;
-  const int t = xcd_remap(blockIdx.x, p.mtiles * p.ntiles);
-  const int mt = t / p.ntiles, nt = t - mt * p.ntiles;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+
+// Many rows: a workgroup of WM x WN waves takes 32 FM WM rows x 32 FN WN outputs.  Codes and scales reach LDS by LDS-DMA,
+// 256 channels a stage -- 128 bytes of a row, a cache line -- and two stages: one is read, the next one lands.
+// The 32 x 32 x 64 form of the matrix instruction, not the 16 x 16 x 128 one: both take the scale operands in an
+// instruction slot of their own, which costs the shorter one more of its rate (a loop of nothing else reaches 9.5
+// against 6.9 PFLOP/s).
+__device__ __forceinline__ int mx_swz(int row) { return (row >> 1) & 7; }     // order of a row's eight 16-byte chunks
+typedef __attribute__((address_space(1))) const void* mxg_t;
+typedef __attribute__((address_space(3))) void* mxl_t;
+// op_sel picks byte U of the scale words
+template <int U> __device__ __forceinline__ f32x16_t mx4_mfma32(u32x4_t a, int sa, u32x4_t b, int sb, f32x16_t acc) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx4_operand(a), mx4_operand(b), acc, 4, 4, U, sa, U, sb);
+}
+
+// A wave's fragments -> out.  acc[i][j] holds outputs 32 i + 8 q + 4 h + (0..3) of row 32 j + r32; they are turned into
+// rows of 128 bytes in the wave's own part of LDS, so that a store covers whole lines.
+template <int DT, int FM, int FN>
+__device__ __forceinline__ void mx4_epilogue(const MxParams& p, long long m0, int n0, const f32x16_t (&acc)[FN][FM], char* img,
+                                             const float* bias, int lane) {
+  constexpr int NI = DT == CSMRI_F32 ? 1 : 2, CE = DT == CSMRI_F32 ? 4 : 8;     // fragments and outputs per 128 / 16 bytes
+  const int r32 = lane & 31, h = lane >> 5;
+#pragma unroll
+  for (int i0 = 0; i0 < FN; i0 += NI) {
+#pragma unroll
+    for (int i = i0; i < i0 + NI; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4_t bv = *(const f32x4_t*)(bias + 32 * i + 8 * q + 4 * h);
+        const int col = (32 * (i - i0) + 8 * q + 4 * h) * (16 / CE);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+          f32x4_t v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = acc[i][j][4 * q + r] + bv[r];
+            v[r] = v[r] > 0.f ? v[r] : v[r] * p.slope;
+            if (n0 + 32 * i + 8 * q + 4 * h + r >= p.N) v[r] = 0.f;
+          }
+          const int row = 32 * j + r32;
+          store4(img + row * 128 + (((col >> 4) ^ (row & 7)) << 4) + (col & 15), 0, DT, v);
+        }
+      }
+    const int ch = lane & 7, n = n0 + 32 * i0 + ch * CE;
+#pragma unroll
+    for (int t = 0; t < FM * 4; ++t) {
+      const int row = t * 8 + (lane >> 3);
+      const u32x4_t v = *(const u32x4_t*)(img + row * 128 + ((ch ^ (row & 7)) << 4));
+      if (m0 + row < p.M && n < p.Npad) *(u32x4_t*)((char*)p.out + ((m0 + row) * p.ops + n) * (16 / CE)) = v;
+    }
+  }
+}
+
+template <int FM, int FN, int WM, int WN, int OCC, bool PP>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxParams p) {
+  constexpr int NW = WM * WN, BM = 32 * FM * WM, BN = 32 * FN * WN, STG = (BM + BN) * 128, SCL = (BM + BN) * 16;
+  constexpr int NA = BM / (8 * NW), NB = BN / (8 * NW), NS = ((BM + BN) / 64 + NW - 1) / NW;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  char* sscl = smem + 2 * STG;                             // scales: two groups of 512 channels, 16 bytes a row
+  float* sbias = (float*)(sscl + 2 * SCL);
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wid / WN, wn = wid % WN, r32 = lane & 31, h = lane >> 5;
+  const int tz = xcd_remap(blockIdx.x, p.mtiles * p.ntiles * p.splits), split = tz / (p.mtiles * p.ntiles);
+  const int t = tz - split * p.mtiles * p.ntiles;
+  const int mt = t / p.ntiles, nt = t - mt * p.ntiles, k0 = split * p.schunk;
   const long long m0 = (long long)mt * BM; const int n0 = nt * BN;
-  // staging: two 16-byte chunks a thread and image; rows behind the end read the last row, their results are not stored
-  const char* xsrc[2]; const char* wsrc[2]; int off[2];
+  const int mrows = p.M - m0 < BM ? (int)(p.M - m0) : BM, nrows = p.N - n0 < BN ? p.N - n0 : BN;
+  const char* xb = p.xq + m0 * p.cb + k0 * 64; const char* wb = p.wq + (long long)n0 * p.cb + k0 * 64;
+  const unsigned char* xsb = p.xs + m0 * p.sb + k0 * 4; const unsigned char* wsb = p.ws + (long long)n0 * p.sb + k0 * 4;
+  // rows behind the end read the tile's last row: their results are not stored.  An LDS-DMA instruction fills 1 KiB (eight
+  // rows) in lane order, so the swizzle of a row's chunks is applied to the source
+  unsigned xo[NA], wo[NB], so[NS];
+  const int drow = wid * 8 + (lane >> 3), dch = (lane & 7) ^ mx_swz(drow);       // (j * NW * 8 rows on: the same swizzle)
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int id = j * 256 + tid, row = id >> 2, ch = id & 3;
-    const long long m = m0 + row < p.M ? m0 + row : p.M - 1;
-    const int n = n0 + row < p.N ? n0 + row : p.N - 1;
-    xsrc[j] = p.xq + m * p.cb + ch * 16;
-    wsrc[j] = p.wq + (long long)n * p.cb + ch * 16;
-    off[j] = mx_off(row, ch);
+  for (int j = 0; j < NA; ++j) { const int row = j * NW * 8 + drow; xo[j] = (unsigned)(row < mrows ? row : mrows - 1) * p.cb + dch * 16; }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) { const int row = j * NW * 8 + drow; wo[j] = (unsigned)(row < nrows ? row : nrows - 1) * p.cb + dch * 16; }
+#pragma unroll
+  for (int j = 0; j < NS; ++j) {
+    const int row = (j * NW + wid) * 64 + lane;            // rows of x, then rows of w
+    so[j] = row < BM ? (unsigned)(row < mrows ? row : mrows - 1) * p.sb
+                     : (unsigned)(row - BM < nrows ? row - BM : nrows - 1) * p.sb;
   }
-  const unsigned char* xsc[4]; const unsigned char* wsc[4];
+  const int K = min(p.schunk, p.ksteps - k0);              // (schunk: whole groups of four, at least one in every split)
+  auto issue = [&](int st) {
+    char* buf = smem + (st & 1) * STG;
+    if ((st & 1) == 0) {
+      char* sd = sscl + ((st >> 1) & 1) * SCL;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long m = m0 + wm * 64 + i * 16 + r16;
-    const int n = n0 + wn * 64 + i * 16 + r16;
-    xsc[i] = p.xs + (m < p.M ? m : p.M - 1) * p.sb + g;
-    wsc[i] = p.ws + (long long)(n < p.N ? n : p.N - 1) * p.sb + g;
-  }
-  f32x4_t acc[4][4];
+      for (int j = 0; j < NS; ++j) {
+        const int first = (j * NW + wid) * 64;
+        if ((BM + BN) % (64 * NW) == 0 || first < BM + BN) {
+          const unsigned char* b = (first < BM ? xsb : wsb) + (st >> 1) * 16;
+          __builtin_amdgcn_global_load_lds((mxg_t)(b + so[j]), (mxl_t)(sd + first * 16), 16, 0, 0);
+        }
+      }
+    }
+    // where only half of the stage is left, the lanes of the other half read that one again
+    const unsigned back = 2 * st + 1 >= K && dch >= 4 ? 64 : 0;
+    const char* xk = xb + st * 128; const char* wk = wb + st * 128;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < NA; ++j)
+      __builtin_amdgcn_global_load_lds((mxg_t)(xk + (xo[j] - back)), (mxl_t)(buf + (j * NW + wid) * 1024), 16, 0, 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < p.ksteps; ++k) {
-    u32x4_t xv[2], wv[2];
+    for (int j = 0; j < NB; ++j)
+      __builtin_amdgcn_global_load_lds((mxg_t)(wk + (wo[j] - back)), (mxl_t)(buf + BM * 128 + (j * NW + wid) * 1024), 16, 0, 0);
+  };
+  // lane (r32, h) feeds channels 128 u + 64 f + 32 h .. + 31 of its row to the instruction (u, f): chunk 4 u + 2 f + h
+  const int foff = r32 * 128 + ((h ^ mx_swz(r32)) << 4);
+  const int xoff = wm * FM * 4096 + foff, woff = BM * 128 + wn * FN * 4096 + foff;
+  const int xsoff = (wm * FM * 32 + r32) * 16, wsoff = (BM + wn * FN * 32 + r32) * 16;
+  const unsigned sel = 0x06040200u + (unsigned)h * 0x01010101u;   // bytes h and 2 + h of two steps' scale words
+  f32x16_t acc[FN][FM];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { xv[j] = *(const u32x4_t*)(xsrc[j] + k * 64); wv[j] = *(const u32x4_t*)(wsrc[j] + k * 64); }
-    int xs[4], ws[4];
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { xs[i] = xsc[i][k * 4]; ws[i] = wsc[i][k * 4]; }
-    __syncthreads();
+    for (int j = 0; j < FM; ++j)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) { *(u32x4_t*)(smem + off[j]) = xv[j]; *(u32x4_t*)(smem + IMG + off[j]) = wv[j]; }
-    __syncthreads();
-    i32x8_t xf[4], wf[4];
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  u32x4_t xf[FM][2], wf[FN][2]; int xs[FM], ws[FN];
+  auto scale_word = [&](const char* a) {
+    const u32x2_t v = *(const u32x2_t*)a;
+    return (int)__builtin_amdgcn_perm(v[1], v[0], sel);
+  };
+  auto load = [&](int s) {                                 // s: step of 128 channels
+    const char* buf = smem + ((s >> 1) & 1) * STG;
+    if ((s & 1) == 0) {                                    // scales of two steps
+      const char* sc = sscl + ((s >> 2) & 1) * SCL + (s & 2) * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xf[i] = mx4_operand(*(const u32x4_t*)(smem + mx_off(wm * 64 + i * 16 + r16, g)));
-      wf[i] = mx4_operand(*(const u32x4_t*)(smem + IMG + mx_off(wn * 64 + i * 16 + r16, g)));
+      for (int i = 0; i < FN; ++i) ws[i] = scale_word(sc + wsoff + i * 512);
+#pragma unroll
+      for (int j = 0; j < FM; ++j) xs[j] = scale_word(sc + xsoff + j * 512);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int f = 0; f < 2; ++f) {
+      const int flip = (s & 1) * 64 + f * 32;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = mx4_mfma(wf[i], ws[i], xf[j], xs[j], acc[i][j]);
+      for (int i = 0; i < FN; ++i) wf[i][f] = *(const u32x4_t*)(buf + ((woff + i * 4096) ^ flip));
+#pragma unroll
+      for (int j = 0; j < FM; ++j) xf[j][f] = *(const u32x4_t*)(buf + ((xoff + j * 4096) ^ flip));
+    }
+  };
+#define MX_MUL(B) \
+    _Pragma("unroll") for (int j = 0; j < FM; ++j) \
+    _Pragma("unroll") for (int i = 0; i < FN; ++i) \
+      acc[i][j] = mx4_mfma32<B>(wf[i][(B) & 1], ws[i], xf[j][(B) & 1], xs[j], acc[i][j]);
+  auto barrier = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const bool late = PP && wm >= WM / 2;
+  issue(0);
+  for (int i = tid; i < BN; i += 64 * NW) sbias[i] = p.bias && p.splits == 1 && n0 + i < p.N ? p.bias[n0 + i] : 0.f;
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  barrier();
+  if (late) barrier();
+  // PP: the two halves of the workgroup alternate, one reads its fragments while the other one multiplies
+#define MX_STEP(U) \
+    { \
+      if (U == 0 && k + 2 < K) issue((k >> 1) + 1); \
+      load(k + U); \
+      if (PP) { \
+        if (U == 1 && late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); \
+        barrier(); \
+      } \
+      __builtin_amdgcn_s_setprio(1); \
+      MX_MUL(2 * U) \
+      MX_MUL(2 * U + 1) \
+      __builtin_amdgcn_s_setprio(0); \
+      if (U == 1 && !(PP && late)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
+      if (PP || U == 1) barrier(); \
+      if (k + U + 1 >= K) break; \
+    }
+  for (int k = 0;; k += 2) {
+    MX_STEP(0)
+    MX_STEP(1)
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const long long m = m0 + wm * 64 + j * 16 + r16;
-    if (m >= p.M) continue;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx4_store(p, m, n0 + wn * 64 + i * 16 + 4 * g, acc[i][j]);
+#undef MX_STEP
+#undef MX_MUL
+  if (PP && !late) barrier();
+  if (!PP) barrier();
+  char* img = smem + wid * FM * 4096;
+  if (p.splits > 1) {
+    MxParams q = p;                                        // a partial sum: no bias, no activation
+    q.out = p.slab + split * p.M * p.Npad; q.ops = p.Npad; q.slope = 1.f;
+    mx4_epilogue<CSMRI_F32, FM, FN>(q, m0 + wm * FM * 32, n0 + wn * FN * 32, acc, img, sbias + wn * FN * 32, lane);
+  } else if (p.out_dt == CSMRI_BF16) mx4_epilogue<CSMRI_BF16, FM, FN>(p, m0 + wm * FM * 32, n0 + wn * FN * 32, acc, img, sbias + wn * FN * 32, lane);
+  else mx4_epilogue<CSMRI_F32, FM, FN>(p, m0 + wm * FM * 32, n0 + wn * FN * 32, acc, img, sbias + wn * FN * 32, lane);
+}
+template <int FM, int FN, int WM, int WN, int OCC, bool PP> static int mx4_gemm_launch(MxParams& p, hipStream_t st) {
+  constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN, LDS = 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16 + BN * 4;
+  static_assert(WM * WN * FM * 4096 <= 2 * (BM + BN) * 128, "the output images share the stages' place");
+  auto kern = mx4_gemm_kernel<FM, FN, WM, WN, OCC, PP>;
+  const long long mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN;
+  if (mt * nt * p.splits > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
+  p.mtiles = (int)mt; p.ntiles = (int)nt;
+  CSMRI_SET_MAX_LDS(kern, LDS);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(mt * nt * p.splits)), dim3(64 * WM * WN), LDS, st, p);
+  CSMRI_LAUNCH_CHECK();
+  return CSMRI_OK;
+}
+
+// split sums -> out, four outputs a thread
+__global__ __launch_bounds__(256) void mx4_join_kernel(const MxParams p) {
+  const int n4 = p.Npad >> 2;
+  const long long total = p.M * n4;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long m = i / n4; const int n = (int)(i - m * n4) * 4;
+    const float* s = p.slab + m * p.Npad + n;
+    f32x4_t v = *(const f32x4_t*)s;
+    for (int z = 1; z < p.splits; ++z) v += *(const f32x4_t*)(s + z * p.M * p.Npad);
+    mx4_store(p, m, n, v);
   }
 }
 
 #define MX4_QUANT_ROWS 16      // up to here the product quantises x itself
-extern "C" size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K) {
-  if (x_dtype == CSMRI_MX4 || rows <= MX4_QUANT_ROWS || K <= 0) return 0;
-  return (size_t)rows * (mx4_code_bytes(K) + mx4_scale_bytes(K));
+#define MX4_SKINNY_ROWS 64     // up to here its rows fit the fragments of one wave
+// Splits of the channels for the tiled kernel: where its 128 x 128 tiles are few and the channels many, until there is a
+// workgroup for each CU; every split keeps 512 channels or more.
+static int mx4_splits(long long rows, int K, int N) {
+  if (rows <= MX4_SKINNY_ROWS) return 1;
+  const long long tiles = ((rows + 127) / 128) * ((N + 127) / 128);
+  const int groups = (K + 511) / 512;
+  if (tiles > 64 || groups < 4) return 1;
+  const int want = (int)(256 / tiles), s = want < groups ? want : groups, per = (groups + s - 1) / s;
+  return (groups + per - 1) / per;
+}
+static size_t mx4_quant_bytes(int x_dtype, long long rows, int K) {
+  return x_dtype == CSMRI_MX4 || rows <= MX4_QUANT_ROWS ? 0 : (size_t)rows * (mx4_code_bytes(K) + mx4_scale_bytes(K));
+}
+extern "C" size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K, int N) {
+  if (rows <= 0 || K <= 0 || N <= 0) return 0;
+  const int s = mx4_splits(rows, K, N);
+  return mx4_quant_bytes(x_dtype, rows, K) + (s > 1 ? (size_t)s * rows * ((N + 7) / 8 * 8) * sizeof(float) : 0);
 }
 
 extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, const uint8_t* x_scales, long long rows, int K,
@@ -304,7 +494,7 @@ extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, co
   CSMRI_CHECK_ARG(x_dtype == CSMRI_MX4 ? true : mx4_shape_ok(rows, K, x_pix_stride, x_dtype));
   if (rows == 0) return CSMRI_OK;
   CSMRI_CHECK_ARG(x && out && (x_dtype != CSMRI_MX4 || x_scales));
-  CSMRI_CHECK_ARG(csmri_mx4_linear_work_bytes(x_dtype, rows, K) == 0 || work);
+  CSMRI_CHECK_ARG(csmri_mx4_linear_work_bytes(x_dtype, rows, K, N) == 0 || work);
   if ((((uintptr_t)w_codes | (uintptr_t)w_scales | (uintptr_t)work | (uintptr_t)x_scales) & 15) ||
       !mx4_rows_aligned(out, out_pix_stride, out_dtype) ||
       (x_dtype == CSMRI_MX4 ? ((uintptr_t)x & 15) != 0 : !mx4_rows_aligned(x, x_pix_stride, x_dtype))) return CSMRI_E_ALIGN;
@@ -323,7 +513,7 @@ extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, co
     const int rc = csmri_mx4_quantize(x_dtype, x, x_pix_stride, rows, K, (void*)p.xq, (uint8_t*)p.xs, stream);
     if (rc != CSMRI_OK) return rc;
   }
-  if (rows <= 64) {
+  if (rows <= MX4_SKINNY_ROWS) {
     const dim3 g((npad + 15) / 16), b(512);
     if (!p.xq) {
       if (x_dtype == CSMRI_F32) hipLaunchKernelGGL((mx4_skinny_kernel<1, CSMRI_F32>), g, b, 0, st, p);
@@ -334,10 +524,15 @@ extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, co
     CSMRI_LAUNCH_CHECK();
     return CSMRI_OK;
   }
-  const long long mt = (rows + 127) / 128, nt = (npad + 127) / 128;
-  if (mt * nt > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
-  p.mtiles = (int)mt; p.ntiles = (int)nt;
-  hipLaunchKernelGGL(mx4_gemm_kernel, dim3((unsigned)(mt * nt)), dim3(256), 0, st, p);
+  p.splits = mx4_splits(rows, K, N);
+  p.schunk = p.splits > 1 ? 4 * (((K + 511) / 512 + p.splits - 1) / p.splits) : p.ksteps;
+  p.slab = (float*)((char*)work + mx4_quant_bytes(x_dtype, rows, K));
+  // the large tile reads each operand half as often and needs a CU to itself: taken once there is one for each CU
+  const long long big = ((rows + 255) / 256) * ((N + 255) / 256);
+  const int rc = big >= 256 ? mx4_gemm_launch<4, 2, 2, 4, 2, false>(p, st) : mx4_gemm_launch<2, 2, 2, 2, 2, false>(p, st);
+  if (rc != CSMRI_OK || p.splits == 1) return rc;
+  const long long blocks = (rows * (npad / 4) + 255) / 256;
+  hipLaunchKernelGGL(mx4_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p);
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }

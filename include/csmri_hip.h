@@ -658,7 +658,7 @@ int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z, int z_pix_
  * dgamma = sum_p dy h, dbeta = sum_p dy.  The input is either x (m and r are computed again) or q8 / s8 with the
  * forward's stats; with the kept form and slope != 1, z is needed for the sign of y (optional otherwise).  dx may be
  * NULL; dgamma and dbeta (both or neither, [C_real], added to where accumulate != 0) need partial:
- * [csmri_ln_bwd_rows(npix, C)][2][C] fp32, 16-byte aligned.  Fixed summation order. */
+ * [csmri_ln_bwd_rows(npix, C)][2][C_real] fp32.  Fixed summation order. */
 int csmri_ln_bwd_rows(long long npix, int C);
 int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const void* x, int x_pix_stride, const void* q8,
                  const uint8_t* s8, const float* stats, const void* z, int z_pix_stride, void* dx, int dx_pix_stride,
@@ -681,7 +681,7 @@ int csmri_act8_restore(const void* q8, const uint8_t* s8, long long npix, int C,
  * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts.
  * splits: csmri_act8_wgrad_splits; slab: csmri_act8_wgrad_slab_bytes (NULL when that is 0).  Fixed summation order.
  * npix == 0 leaves zeros (or what was there, with accumulate). */
-int csmri_act8_wgrad_splits(long long npix, int Cout, int Cin);
+int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin);
 size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real);
 int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride, const void* q8, const uint8_t* s8, long long npix,
                      int Cout, int Cin, int Cout_real, int Cin_real, int splits, float* slab, float* dw, float* db,
@@ -705,7 +705,7 @@ int csmri_mx4_dequantize(const void* codes, const uint8_t* scales, long long row
  * n < N; channels N..8 ceil(N / 8) of out are written as zeros (out_pix_stride covers them).  x: fp32 / bf16 pixels,
  * quantised on the way, or codes (x_dtype CSMRI_MX4, with x_scales; x_pix_stride unused).  w: N rows of K channels.
  * work: csmri_mx4_linear_work_bytes bytes, 16-byte aligned (NULL when that is 0).  bias may be NULL. */
-size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K);
+size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K, int N);
 int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, const uint8_t* x_scales, long long rows, int K,
                      const void* w_codes, const uint8_t* w_scales, int N, const float* bias, float slope, void* out,
                      int out_dtype, int out_pix_stride, void* work, void* stream);

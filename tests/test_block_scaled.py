@@ -114,7 +114,7 @@ def test_entry_points_refuse_bad_arguments():
   assert bw_with(_3=None, _5=p, _6=p) == ARG                                # kept input without statistics
   assert bw_with(_3=None, _5=p, _6=p, _7=p, _17=0.1) == ARG                 # ... and no sign
   assert bw_with(_18=None) == ARG and bw_with(_20=None) == ARG and bw_with(_15=None) == ARG
-  assert bw_with(_10=p) == ARG and bw_with(_18=p + 4) == ALI
+  assert bw_with(_10=p) == ARG and bw_with(_15=p + 4) == ALI
   sv, rs = raw('csmri_act8_save'), raw('csmri_act8_restore')
   assert sv(0, None, 16, 0, 16, None, None, None) == 0 and rs(None, None, 0, 16, 0, None, 16, None) == 0
   assert sv(0, p, 16, 4, 12, p, p, None) == ARG and sv(3, p, 16, 4, 16, p, p, None) == ARG and sv(0, p, 8, 4, 16, p, p, None) == ARG
@@ -127,7 +127,7 @@ def test_entry_points_refuse_bad_arguments():
   assert wg(0, p, 16, p, p, 4, 16, 16, 16, 16, 5, p, p, None, 0, None) == ARG             # more splits than pixels
   assert wg(0, p + 4, 16, p, p, 4, 16, 16, 16, 16, 1, None, p, None, 0, None) == ALI
   assert wg(1, p, 20, p, p, 4, 16, 16, 16, 16, 1, None, p, None, 0, None) == ALI
-  assert raw('csmri_act8_wgrad_splits')(0, 16, 16) == 1 and raw('csmri_act8_wgrad_splits')(100, 16, 16) == 1
+  assert raw('csmri_act8_wgrad_splits')(0, 0, 16, 16) == 1 and raw('csmri_act8_wgrad_splits')(1, 100, 16, 16) == 1
   assert raw('csmri_act8_wgrad_slab_bytes')(3, 5, 7) == 3 * 40 * 4 and raw('csmri_act8_wgrad_slab_bytes')(1, 5, 7) == 0
   assert [raw('csmri_mx4_code_bytes')(k) for k in (0, 8, 128, 136, 4096)] == [0, 64, 64, 128, 2048]
   assert [raw('csmri_mx4_scale_bytes')(k) for k in (0, 8, 512, 520, 4096)] == [0, 16, 16, 32, 128]
@@ -148,7 +148,7 @@ def test_entry_points_refuse_bad_arguments():
   assert li_with(_0=4) == ARG                                               # codes without scales
   assert li_with(_4=200) == ARG                                             # quantised x has nowhere to go
   assert li_with(_1=p + 2) == ALI and li_with(_7=p + 1) == ALI and li_with(_13=25, _12=1) == ALI
-  assert raw('csmri_mx4_linear_work_bytes')(1, 200, 136) == 200 * (128 + 16) and raw('csmri_mx4_linear_work_bytes')(4, 200, 136) == 0
+  assert raw('csmri_mx4_linear_work_bytes')(1, 200, 136, 24) == 200 * (128 + 16) and raw('csmri_mx4_linear_work_bytes')(4, 200, 136, 24) == 0
 
 
 def test_operators_refuse_host_tensors_and_shapes():
@@ -338,7 +338,7 @@ def test_weight_gradient_from_kept_activations(ops, n, cin, cout, dtype):
   g = gy.double()[:, :cout]
   dw, db = ops.act8_wgrad(a, gy.cuda(), cout, cin_real)
   assert dw.shape == (cout, cin_real) and db.shape == (cout,)
-  splits = ops.lib.raw('csmri_act8_wgrad_splits')(n, pad8(cout), cin)
+  splits = ops.lib.raw('csmri_act8_wgrad_splits')(ops.dt_of(gy), n, pad8(cout), cin)
   parts = 3 if dtype == torch.float32 else 1
   L = 2 * parts * (n / splits / 32 + 1 + 32) + splits / 64 + 8
   close(dw, g.t() @ xr, (L + 1) * U * (g.abs().t() @ xr.abs()) + 1e-300, 'dw')
