@@ -4,6 +4,7 @@
 // Save and restore are streams: one read, one write, bound by HBM.
 #include "micro.h"
 #include "wgrad_params.h"
+#include <type_traits>
 
 template <int DT>
 __global__ __launch_bounds__(256) void act8_save_kernel(const void* __restrict__ x, int ps, long long rows, int c8,
@@ -199,107 +200,105 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
   }
 }
 
-__device__ __attribute__((aligned(16))) char a8_zero_page[16];
-typedef __attribute__((address_space(1))) const void* a8g_t;
-typedef __attribute__((address_space(3))) void* a8l_t;
-
 // A workgroup of WN x WC waves takes a tile of 16 FN WN output x 16 FC WC input channels over a range of pixels, KP at a
-// time.  A bf16 dY goes to LDS by LDS-DMA into a ring of three stages; the kept input passes through registers, where
-// its codes become bf16, into one of two; what is loaded during step k is waited for in step k + 1, needed in step k + 2.
-template <int DT, int FN, int FC, int WN, int WC>
+// time.  Both operands pass through registers into one of two LDS stages, the input's codes becoming bf16 on the way, and
+// are loaded a step ahead of that.  (LDS-DMA would spare dY the registers, but the compiler lets no transposed read pass a
+// pending one; a second set of registers, to load two steps ahead, costs more in occupancy than it hides.)  Bound by the
+// matrix unit and the steps around it: of the 192 us at 2048 x 2048 channels and 16384 pixels, a loop of the products,
+// barriers and stores alone takes 132.
+template <int DT, int FN, int FC, int WN, int WC, int KP>
 __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WParams p) {
-  constexpr int NW = WN * WC, NT = 64 * NW, BN = 16 * FN * WN, BC = 16 * FC * WC, KP = 32, CN = BN / 8, CC = BC / 8;
-  constexpr bool SPLIT = DT == CSMRI_F32;
-  constexpr int PL = SPLIT ? 3 : 1, YST = SPLIT ? 2 : 3;         // planes of dY, stages of dY
-  constexpr int YIMG = KP * BN * 2, XIMG = KP * BC * 2;
-  constexpr int NY = KP * CN / NT, NX = KP * CC / NT;            // 16-byte chunks (eight channels) a thread and stage
+  constexpr int NW = WN * WC, NT = 64 * NW, BN = 16 * FN * WN, BC = 16 * FC * WC, CN = BN / 8, CC = BC / 8;
+  constexpr int PL = DT == CSMRI_F32 ? 3 : 1, ES = DT == CSMRI_F32 ? 4 : 2;
+  constexpr int YIMG = KP * BN * 2, XIMG = KP * BC * 2, STG = PL * YIMG + XIMG;
+  constexpr int NY = KP * CN / NT, NX = KP * CC / NT;            // chunks of eight channels a thread and stage
   static_assert(KP * CN % NT == 0 && KP * CC % NT == 0, "whole chunks per thread");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  char* ximg = smem + YST * PL * YIMG;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid / WC, wc = wid % WC;
   const int tiles = p.ntiles * p.ctiles;
-  const int tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
+  // an XCD takes neighbouring tiles of the same pixels, which then meet in its L2
+  const int wg = xcd_remap(blockIdx.x, tiles * p.splits), split = wg / tiles, tile = wg - split * tiles;
   const int nt = tile / p.ctiles, ct = tile - nt * p.ctiles;
   const int n0 = nt * BN, c0 = ct * BC;
   const long long pb = split * p.chunk, pe = pb + p.chunk < p.npix ? pb + p.chunk : p.npix;
   const int sblocks = (p.Cin + MICRO_BLOCK - 1) / MICRO_BLOCK;
   const int steps = pe > pb ? (int)((pe - pb + KP - 1) / KP) : 0;
 
-  f32x4_t acc[FN][FC], accb[FN];
+  constexpr int NB = FN / WC;                                     // fragments whose column sums a wave takes
+  static_assert(FN % WC == 0, "every wave of a row takes as many");
+  f32x4_t acc[FN][FC], accb[NB];
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
-    accb[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < FC; ++j) acc[i][j] = accb[i];
+    for (int j = 0; j < FC; ++j) acc[i][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
-  const bool want_b = p.db && ct == 0 && wc == 0;
-  const bf16x8_t ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
+#pragma unroll
+  for (int i = 0; i < NB; ++i) accb[i] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 
-  // chunk j of a thread: slot (row, place) of the image in thread order; the swizzle puts another chunk of the row there
-  const char* yp[NY]; int yrow[NY]; bool yok[NY];
+  // chunk j of a thread: row (j NT + tid) / chunks of a row.  Channels behind the end read the first ones (their results are
+  // not stored), pixels behind the range its last one, with a dY of zero
+  int yrow[NY], yoff[NY], xrow[NX], xoff[NX], ych[NY], xch[NX];
 #pragma unroll
   for (int j = 0; j < NY; ++j) {
-    const int id = (j * NW + wid) * 64 + lane, row = id / CN, place = id % CN;
-    const int ch = (img_off<CN>(row, place) >> 4) % CN;
-    yrow[j] = row; yok[j] = n0 + ch * 8 < p.Cout;
-    yp[j] = p.dy + ((pb + row) * p.dyps + n0 + ch * 8) * (SPLIT ? 4 : 2);
+    const int id = j * NT + tid, ch = id % CN;
+    yrow[j] = id / CN; yoff[j] = img_off<CN>(yrow[j], ch); ych[j] = (n0 + ch * 8 < p.Cout ? n0 + ch * 8 : 0) * ES;
   }
-  const unsigned char* xp[NX]; const unsigned char* sp[NX]; int xrow[NX]; bool xok[NX]; int xoff[NX];
 #pragma unroll
   for (int j = 0; j < NX; ++j) {
-    const int id = j * NT + tid, row = id / CC, ch = id % CC;
-    xrow[j] = row; xok[j] = c0 + ch * 8 < p.Cin;
-    xp[j] = p.q + (pb + row) * p.Cin + c0 + ch * 8;
-    sp[j] = p.s + (pb + row) * sblocks + ((c0 + ch * 8) >> 5);
-    xoff[j] = img_off<CC>(row, ch);
+    const int id = j * NT + tid, ch = id % CC;
+    xrow[j] = id / CC; xoff[j] = img_off<CC>(xrow[j], ch); xch[j] = c0 + ch * 8 < p.Cin ? c0 + ch * 8 : 0;
   }
-  const long long ystep = (long long)KP * p.dyps * (SPLIT ? 4 : 2), xstep = (long long)KP * p.Cin, sstep = (long long)KP * sblocks;
-  raw8<DT> yv[SPLIT ? NY : 1]; u32x2_t xv[NX]; unsigned sv[NX];
-  auto fetch = [&](int k) {                       // loads of step k; pixels behind the range and channels behind the end: zeros
-    const int left = (int)(pe - pb - (long long)k * KP < KP ? pe - pb - (long long)k * KP : KP);
+  raw8<DT> yv[2][NY]; u32x2_t xv[2][NX]; unsigned sv[2][NX];
+  auto left_of = [&](int k) { const long long l = pe - pb - (long long)k * KP; return l < KP ? (int)l : KP; };
+  // (behind the last step: the last one again, not used)
+  auto fetch = [&](int k, int b) {
+    k = min(k, steps - 1);
+    const long long pix = pb + (long long)k * KP;
+    const char* yb = p.dy + pix * p.dyps * ES;
+    const unsigned char* xb = p.q + pix * p.Cin; const unsigned char* sb = p.s + pix * sblocks;
+    const int last = left_of(k) - 1;
 #pragma unroll
-    for (int j = 0; j < NY; ++j) {
-      const char* src = yp[j] + k * ystep;
-      const bool ok = yok[j] && yrow[j] < left;
-      if constexpr (SPLIT) {
-        yv[j] = raw8<DT>{};
-        if (ok) yv[j] = ldraw8<DT>(src, 0);
-      } else {
-        __builtin_amdgcn_global_load_lds((a8g_t)(ok ? src : a8_zero_page), (a8l_t)(smem + (k % 3) * YIMG + (j * NW + wid) * 1024), 16, 0, 0);
-      }
-    }
+    for (int j = 0; j < NY; ++j) yv[b][j] = ldraw8<DT>(yb + (unsigned)(min(yrow[j], last) * p.dyps * ES + ych[j]), 0);
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
-      const bool ok = xok[j] && xrow[j] < left;
-      xv[j] = *(const u32x2_t*)(ok ? (const char*)xp[j] + k * xstep : a8_zero_page);
-      sv[j] = *(const unsigned char*)(ok ? (const char*)sp[j] + k * sstep : a8_zero_page);
+      const int r = min(xrow[j], last);
+      xv[b][j] = *(const u32x2_t*)(xb + (unsigned)(r * p.Cin + xch[j]));
+      sv[b][j] = sb[(unsigned)(r * sblocks + (xch[j] >> 5))];
     }
   };
-  auto place = [&](int k) {                       // what went through registers -> LDS
-    if constexpr (SPLIT) {
+  auto place = [&](int k, int b) {
+    char* yi = smem + (k & 1) * STG; char* xi = yi + PL * YIMG;
+    const int left = left_of(k);
+    if (left < KP) {
 #pragma unroll
-      for (int j = 0; j < NY; ++j) {
+      for (int j = 0; j < NY; ++j)
+        if (yrow[j] >= left) yv[b][j] = raw8<DT>{};
+    }
+#pragma unroll
+    for (int j = 0; j < NY; ++j) {
+      if constexpr (DT == CSMRI_F32) {
         float f[8]; u32x4_t o[3];
-        cvt8<DT>(yv[j], f);
+        cvt8<DT>(yv[b][j], f);
         split3(f, o);
-        char* dst = smem + (k & 1) * PL * YIMG + (j * NW + wid) * 1024 + lane * 16;
 #pragma unroll
-        for (int i = 0; i < 3; ++i) *(u32x4_t*)(dst + i * YIMG) = o[i];
+        for (int i = 0; i < 3; ++i) *(u32x4_t*)(yi + i * YIMG + yoff[j]) = o[i];
+      } else {
+        *(u32x4_t*)(yi + yoff[j]) = yv[b][j].a;
       }
     }
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
-      const float s = __uint_as_float(sv[j] << 23);
+      const float s = __uint_as_float(sv[b][j] << 23);
       u32x4_t o;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        o[2 * q] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, false));
-        o[2 * q + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, true));
+        o[2 * q] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[b][j][q], s, false));
+        o[2 * q + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[b][j][q], s, true));
       }
-      *(u32x4_t*)(ximg + (k & 1) * XIMG + xoff[j]) = o;
+      *(u32x4_t*)(xi + xoff[j]) = o;
     }
   };
-  auto barrier = [&]() {
+  auto barrier = [&]() {                          // (not __syncthreads: that would wait for the loads under way too)
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
@@ -309,36 +308,50 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
   // fragments: a 16-lane group reads 4 pixel rows x 16 channels; rows 8 g + (0..3) and 8 g + (4..7) of the step
   const int g = lane >> 4, tr = (lane & 15) >> 2, tc = lane & 3, lo = 8 * g + tr, hi = lo + 4;
   const int yc = wn * FN * 2 + (tc >> 1), xc = wc * FC * 2 + (tc >> 1), in = (tc & 1) * 8;
-  auto multiply = [&](int k) {
-    const char* yi = smem + (SPLIT ? (k & 1) * PL : k % 3) * YIMG;
-    const char* xi = ximg + (k & 1) * XIMG;
-    bf16x8_t xf[FC];
+  const bf16x8_t ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
+  const bool want_b = p.db && ct == 0;
+  auto run = [&](auto with_bias) {
+    auto multiply = [&](int k) {
+      const char* yi = smem + (k & 1) * STG; const char* xi = yi + PL * YIMG;
 #pragma unroll
-    for (int j = 0; j < FC; ++j) xf[j] = tr_frag(xi, img_off<CC>(lo, xc + 2 * j) + in, img_off<CC>(hi, xc + 2 * j) + in);
+      for (int kk = 0; kk < KP; kk += 32) {
+        bf16x8_t xf[FC];
 #pragma unroll
-    for (int pl = 0; pl < PL; ++pl)
+        for (int j = 0; j < FC; ++j) xf[j] = tr_frag(xi, img_off<CC>(kk + lo, xc + 2 * j) + in, img_off<CC>(kk + hi, xc + 2 * j) + in);
 #pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const bf16x8_t yf = tr_frag(yi + pl * YIMG, img_off<CN>(lo, yc + 2 * i) + in, img_off<CN>(hi, yc + 2 * i) + in);
+        for (int pl = 0; pl < PL; ++pl)
 #pragma unroll
-        for (int j = 0; j < FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, xf[j], acc[i][j], 0, 0, 0);
-        if (want_b) accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, ones, accb[i], 0, 0, 0);
+        for (int i = 0; i < FN; ++i) {
+          const bf16x8_t yf = tr_frag(yi + pl * YIMG, img_off<CN>(kk + lo, yc + 2 * i) + in, img_off<CN>(kk + hi, yc + 2 * i) + in);
+#pragma unroll
+          for (int j = 0; j < FC; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, xf[j], acc[i][j], 0, 0, 0);
+        }
+        if constexpr (decltype(with_bias)::value) {
+#pragma unroll
+          for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const int c = yc + 2 * (wc * NB + i);
+            const bf16x8_t yf = tr_frag(yi + pl * YIMG, img_off<CN>(kk + lo, c) + in, img_off<CN>(kk + hi, c) + in);
+            accb[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, ones, accb[i], 0, 0, 0);
+          }
+        }
       }
-  };
-  if (steps > 0) {
-    fetch(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    place(0);
-    fetch(1);
+    };
+    if (steps == 0) return;
+    fetch(0, 0);
+    place(0, 0);
+    fetch(1, 0);
     for (int k = 0; k < steps; ++k) {
       barrier();                                  // stage k is there for everyone; everyone has read stage k - 1
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      place(k + 1);
-      fetch(k + 2);
+      place(k + 1, 0);
+      fetch(k + 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
       multiply(k);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  }
+  };
+  if (want_b) run(std::true_type{});
+  else run(std::false_type{});
   // lane l holds rows n = 4 g + r, column c = l & 15 of each fragment
   const long long len = (long long)p.Cout_real * p.Cin_real;
   float* dw = p.splits > 1 ? p.slab + split * (len + p.Cout_real) : p.dw;
@@ -358,39 +371,50 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
 #pragma unroll
       for (int j = 0; j < FC; ++j)
         if (cb + 16 * j < p.Cin_real) o[16 * j] = acc[i][j][r] + old[j];
-      if (want_b && (lane & 15) == 0) db[n] = accb[i][r] + (add ? db[n] : 0.f);
     }
+  if (want_b && (lane & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = n0 + (wn * FN + wc * NB + i) * 16 + 4 * g + r;
+        if (n < p.Cout_real) db[n] = accb[i][r] + (add ? db[n] : 0.f);
+      }
+  }
 }
 
-// tile: 64 or 128 a side by the channel counts, 256 x 256 where that still fills half the chip's CUs with one split each
+// Tile: 64 or 128 a side by the channel counts, two workgroups a CU; 256 x 256 (an fp32 dY's three planes do not fit it),
+// which reads LDS a third less per product, where 2048 pixels a split still leave three quarters of the CUs a workgroup.
+// 2048 x 2048 channels, 16384 pixels: 192 us against 225 with 128 x 128; 512 x 512, 8192 pixels: 46 against 35.
 struct A8WTile { int bn, bc; };
-static A8WTile a8w_tile(int dtype, long long npix, int Cout, int Cin) {
-  if (dtype == CSMRI_BF16 && (long long)cdiv(Cout, 256) * cdiv(Cin, 256) * (npix / 2048) >= 128 && Cout > 128 && Cin > 128)
-    return {256, 256};
+static A8WTile a8w_tile(int dy_dtype, long long npix, int Cout, int Cin) {
+  if (dy_dtype == CSMRI_BF16 && Cout > 128 && Cin > 128 &&
+      (long long)cdiv(Cout, 256) * cdiv(Cin, 256) * (npix / 2048) >= 192) return {256, 256};
   return {Cout <= 64 ? 64 : 128, Cin <= 64 ? 64 : 128};
 }
 extern "C" int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin) {
   if (npix <= 0 || Cout <= 0 || Cin <= 0) return 1;
   const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
   const long long tiles = (long long)cdiv(Cout, t.bn) * cdiv(Cin, t.bc);
-  // one workgroup of the large tile a CU, two of the others; at least sixteen steps each
   long long s = (t.bn == 256 ? 256 : 512) / tiles;
-  const long long most = npix / 512;
+  const long long most = npix / 512;                          // at least eight or sixteen steps each
   if (s > most) s = most;
   return s < 1 ? 1 : (int)s;
 }
-template <int DT, int FN, int FC, int WN, int WC> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
-  constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = 32 * 2 * (BN * (DT == CSMRI_F32 ? 6 : 3) + BC * 2);
-  auto kern = act8_wgrad_kernel<DT, FN, FC, WN, WC>;
+template <int DT, int FN, int FC, int WN, int WC, int KP> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
+  constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = 2 * KP * 2 * (BN * (DT == CSMRI_F32 ? 3 : 1) + BC);
+  auto kern = act8_wgrad_kernel<DT, FN, FC, WN, WC, KP>;
   CSMRI_SET_MAX_LDS(kern, LDS);
   hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WN * WC), LDS, st, p);
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }
+// pixels a step: 64, for fewer barriers, where two stages of that fit two workgroups into a CU's LDS
 template <int DT> static int a8w_dispatch(const A8WTile& t, const A8WParams& p, unsigned grid, hipStream_t st) {
-  if constexpr (DT == CSMRI_BF16) if (t.bn == 256) return a8w_launch<DT, 8, 4, 2, 4>(p, grid, st);
-  if (t.bn == 128) return t.bc == 128 ? a8w_launch<DT, 4, 4, 2, 2>(p, grid, st) : a8w_launch<DT, 4, 2, 2, 2>(p, grid, st);
-  return t.bc == 128 ? a8w_launch<DT, 2, 4, 2, 2>(p, grid, st) : a8w_launch<DT, 2, 2, 2, 2>(p, grid, st);
+  constexpr int KP = DT == CSMRI_F32 ? 32 : 64;
+  if constexpr (DT == CSMRI_BF16) if (t.bn == 256) return a8w_launch<DT, 8, 4, 2, 4, 32>(p, grid, st);
+  if (t.bn == 128) return t.bc == 128 ? a8w_launch<DT, 4, 4, 2, 2, KP>(p, grid, st) : a8w_launch<DT, 4, 2, 2, 2, KP>(p, grid, st);
+  return t.bc == 128 ? a8w_launch<DT, 2, 4, 2, 2, KP>(p, grid, st) : a8w_launch<DT, 2, 2, 2, 2, KP>(p, grid, st);
 }
 extern "C" size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real) {
   return splits > 1 ? (size_t)splits * ((size_t)Cout_real * Cin_real + Cout_real) * sizeof(float) : 0;
@@ -413,9 +437,10 @@ extern "C" int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride,
   const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
   p.ntiles = cdiv(Cout, t.bn); p.ctiles = cdiv(Cin, t.bc);
   p.splits = splits; p.slab = slab; p.dw = dw; p.db = db; p.accumulate = accumulate;
-  p.chunk = ((npix + splits - 1) / splits + 31) / 32 * 32;
+  p.chunk = ((npix + splits - 1) / splits + 63) / 64 * 64;
   const long long grid = (long long)p.ntiles * p.ctiles * splits;
-  if (grid > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
+  // offsets inside a step are 32 bits
+  if (grid > 0x7fffffff || (long long)dy_pix_stride * 4 * 32 > 0x7fffffff || (long long)Cin * 32 > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
   const int rc = dy_dtype == CSMRI_F32 ? a8w_dispatch<CSMRI_F32>(t, p, (unsigned)grid, st)
                                        : a8w_dispatch<CSMRI_BF16>(t, p, (unsigned)grid, st);
   if (rc != CSMRI_OK || splits == 1) return rc;
