@@ -28,25 +28,28 @@ struct LNParams {
   float* partial;                                      // backward: [gridDim.x][2][C_real], NULL when neither is wanted
 };
 
-// sum over the lanes of a row
-template <bool WG> __device__ __forceinline__ float row_sum(float a, int group, float* red) {
+// Sums over the lanes of a row.  A workgroup's four waves meet in one of two places of `red`, taken in turn, so that one
+// barrier a sum is enough.
+template <bool WG, int N> __device__ __forceinline__ void row_sums(float (&v)[N], int group, float (*red)[4 * 4], int& turn) {
+  group_sums(v, WG ? 64 : group);
   if constexpr (WG) {
+    static_assert(N <= 4, "places in red");
+    float* r = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
+      for (int i = 0; i < N; ++i) r[(threadIdx.x >> 6) * 4 + i] = v[i];
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-  } else {
-    for (int o = group >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
-    return a;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (r[i] + r[4 + i]) + (r[8 + i] + r[12 + i]);
   }
 }
 
 // mean and 1 / std of U rows held as V vectors a lane; nv[j]: real channels of vector j
 template <bool WG, int V, int U>
-__device__ __forceinline__ void row_stats(const float (&x)[U][V][8], const int (&nv)[V], const LNParams& p, float* red,
-                                          float (&mean)[U], float (&inv)[U]) {
+__device__ __forceinline__ void row_stats(const float (&x)[U][V][8], const int (&nv)[V], const LNParams& p, float (*red)[16],
+                                          int& turn, float (&mean)[U], float (&inv)[U]) {
   const float rc = 1.f / (float)p.C_real;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -57,19 +60,20 @@ __device__ __forceinline__ void row_stats(const float (&x)[U][V][8], const int (
       for (int k = 0; k < 8; ++k) a += k < nv[j] ? x[u][j][k] : 0.f;
     mean[u] = a;
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) mean[u] = row_sum<WG>(mean[u], p.group, red) * rc;
+  row_sums<WG, U>(mean, p.group, red, turn);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
+    mean[u] *= rc;
     float a = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) { const float d = x[u][j][k] - mean[u]; a += k < nv[j] ? d * d : 0.f; }
+      for (int k = 0; k < 8; ++k) { const float d = k < nv[j] ? x[u][j][k] - mean[u] : 0.f; a = __builtin_fmaf(d, d, a); }
     inv[u] = a;
   }
+  row_sums<WG, U>(inv, p.group, red, turn);
 #pragma unroll
-  for (int u = 0; u < U; ++u) inv[u] = rsqrtf(row_sum<WG>(inv[u], p.group, red) * rc + p.eps);
+  for (int u = 0; u < U; ++u) inv[u] = rsqrtf(inv[u] * rc + p.eps);
 }
 
 // the affine step, spelled out so that the forward and the backward's sign test round alike
@@ -81,19 +85,35 @@ template <int V> __device__ __forceinline__ void ld_affine(const float* p, const
 #pragma unroll
     for (int k = 0; k < 8; ++k) o[j][k] = k < nv[j] ? p[c[j] + k] : 0.f;
 }
-
-template <int DT, bool WG, int V, int U, bool KEEP>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
-  __shared__ float red[4];
-  const int gl = WG ? threadIdx.x : (threadIdx.x & (p.group - 1));
-  const int gpw = WG ? 1 : 256 / p.group, gi = WG ? 0 : threadIdx.x / p.group;
-  int c[V], nv[V];
+template <int V> __device__ __forceinline__ void ln_channels(const LNParams& p, int gl, int (&c)[V], int (&nv)[V]) {
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     c[j] = (j * p.group + gl) * 8;
     const int n = p.C_real - c[j];
     nv[j] = n < 0 ? 0 : (n > 8 ? 8 : n);
   }
+}
+
+template <int DT, bool WG, int V, int U, bool KEEP>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
+  __shared__ float red[2][16];
+  int turn = 0;
+  const int gl = WG ? threadIdx.x : (threadIdx.x & (p.group - 1));
+  const int gpw = WG ? 1 : 256 / p.group, gi = WG ? 0 : threadIdx.x / p.group;
+  int c[V], nv[V];
+  ln_channels<V>(p, gl, c, nv);
+  const long long step = (long long)gridDim.x * gpw, first = (long long)blockIdx.x * gpw + gi;
+  raw8<DT> raw[U][V];
+  auto fetch = [&](long long row) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        raw[u][j] = raw8<DT>{};
+        if (c[j] < p.C && row + u * step < p.rows) raw[u][j] = ldraw8<DT>(p.x, (row + u * step) * p.xps + c[j]);
+      }
+  };
+  fetch(first);
   float ga[V][8], be[V][8];
   ld_affine<V>(p.gamma, c, nv, ga);
   ld_affine<V>(p.beta, c, nv, be);
@@ -103,23 +123,16 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
       if (c[j] < p.C) { st8<CSMRI_F32>(p.snap, c[j], ga[j]); st8<CSMRI_F32>(p.snap, p.C + c[j], be[j]); }
   }
   const int sblocks = (p.C + MICRO_BLOCK - 1) / MICRO_BLOCK;
-  const long long step = (long long)gridDim.x * gpw;
-  for (long long row = (long long)blockIdx.x * gpw + gi; row - gi < p.rows; row += step * U) {
-    raw8<DT> raw[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        raw[u][j] = raw8<DT>{};
-        if (c[j] < p.C && row + u * step < p.rows) raw[u][j] = ldraw8<DT>(p.x, (row + u * step) * p.xps + c[j]);
-      }
-    __builtin_amdgcn_sched_barrier(0);
+  const bool act = p.slope != 1.f;
+  for (long long row = first; row - gi < p.rows; row += step * U) {
     float x[U][V][8], mean[U], inv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) cvt8<DT>(raw[u][j], x[u][j]);
-    row_stats<WG, V, U>(x, nv, p, red, mean, inv);
+    fetch(row + step * U);                           // the next rows come in under this one's arithmetic
+    __builtin_amdgcn_sched_barrier(0);
+    row_stats<WG, V, U>(x, nv, p, red, turn, mean, inv);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long rr = row + u * step;
@@ -137,11 +150,13 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
         }
         float o[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const float y = ln_affine((x[u][j][k] - mean[u]) * inv[u], ga[j][k], be[j][k]);
-          const float z = y > 0.f ? y : y * p.slope;
-          o[k] = k < nv[j] ? z : 0.f;
+        for (int k = 0; k < 8; ++k) o[k] = ln_affine((x[u][j][k] - mean[u]) * inv[u], ga[j][k], be[j][k]);
+        if (act) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) o[k] = o[k] > 0.f ? o[k] : o[k] * p.slope;
         }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = k < nv[j] ? o[k] : 0.f;
         if (live && c[j] < p.C) st8<DT>(p.out, rr * p.ops + c[j], o);
       }
       if (live && gl == 0 && p.stats_out) { p.stats_out[rr] = mean[u]; p.stats_out[p.rows + rr] = inv[u]; }
@@ -152,36 +167,26 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
 // KEPT: the input comes as e4m3 codes, with the forward's mean and 1 / std
 template <int DT, bool WG, int V, int U, bool KEPT>
 __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
-  extern __shared__ __attribute__((aligned(16))) float lds[];      // [4] for row_sum, then the affine partials
-  float* red = lds;
+  extern __shared__ __attribute__((aligned(16))) float lds[];      // the affine partials of a workgroup
+  __shared__ float red[2][16];
+  int turn = 0;
   const int gl = WG ? threadIdx.x : (threadIdx.x & (p.group - 1));
   const int gpw = WG ? 1 : 256 / p.group, gi = WG ? 0 : threadIdx.x / p.group;
   int c[V], nv[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    c[j] = (j * p.group + gl) * 8;
-    const int n = p.C_real - c[j];
-    nv[j] = n < 0 ? 0 : (n > 8 ? 8 : n);
-  }
-  float ga[V][8], dg[V][8], db[V][8];
-  ld_affine<V>(p.gamma, c, nv, ga);
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) dg[j][k] = db[j][k] = 0.f;
+  ln_channels<V>(p, gl, c, nv);
   const int sblocks = (p.C + MICRO_BLOCK - 1) / MICRO_BLOCK;
   const float rc = 1.f / (float)p.C_real;
   const bool gate_z = p.slope != 1.f && p.z, gate_x = p.slope != 1.f && !p.z;
-  const long long step = (long long)gridDim.x * gpw;
-  for (long long row = (long long)blockIdx.x * gpw + gi; row - gi < p.rows; row += step * U) {
-    raw8<DT> rx[U][V], rg[U][V], rz[U][V];
-    u32x2_t rq[U][V]; unsigned char rs[U][V];
-    float mean[U], inv[U];
+  const long long step = (long long)gridDim.x * gpw, first = (long long)blockIdx.x * gpw + gi;
+  raw8<DT> rx[U][V], rg[U][V];
+  u32x2_t rq[U][V]; unsigned char rs[U][V];
+  float rm[U], ri[U];
+  auto fetch = [&](long long row) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long rr = row + u * step;
       const bool live = rr < p.rows;
-      if constexpr (KEPT) { mean[u] = live ? p.stats_in[rr] : 0.f; inv[u] = live ? p.stats_in[p.rows + rr] : 0.f; }
+      if constexpr (KEPT) { rm[u] = live ? p.stats_in[rr] : 0.f; ri[u] = live ? p.stats_in[p.rows + rr] : 0.f; }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         rg[u][j] = raw8<DT>{};
@@ -197,66 +202,82 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
         }
       }
     }
-    if (gate_z) {
+  };
+  fetch(first);
+  float ga[V][8], dg[V][8], db[V][8];
+  ld_affine<V>(p.gamma, c, nv, ga);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+  for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          rz[u][j] = raw8<DT>{};
-          if (c[j] < p.C && row + u * step < p.rows) rz[u][j] = ldraw8<DT>(p.z, (row + u * step) * p.zps + c[j]);
-        }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    float x[U][V][8];
+    for (int k = 0; k < 8; ++k) dg[j][k] = db[j][k] = 0.f;
+  for (long long row = first; row - gi < p.rows; row += step * U) {
+    float x[U][V][8], t[U][V][8], mean[U], inv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         if constexpr (KEPT) micro_unpack8(rq[u][j], micro_scale(rs[u][j]), x[u][j]);
         else cvt8<DT>(rx[u][j], x[u][j]);
+        cvt8<DT>(rg[u][j], t[u][j]);
+        if constexpr (KEPT) { mean[u] = rm[u]; inv[u] = ri[u]; }
       }
-    if constexpr (!KEPT) row_stats<WG, V, U>(x, nv, p, red, mean, inv);
+    if (gate_z) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          raw8<DT> rz = raw8<DT>{};
+          if (c[j] < p.C && row + u * step < p.rows) rz = ldraw8<DT>(p.z, (row + u * step) * p.zps + c[j]);
+          float z[8];
+          cvt8<DT>(rz, z);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) t[u][j][k] *= z[k] > 0.f ? 1.f : p.slope;
+        }
+    }
+    fetch(row + step * U);                           // the next rows come in under this one's arithmetic
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!KEPT) row_stats<WG, V, U>(x, nv, p, red, turn, mean, inv);
+    float s[2 * U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long rr = row + u * step;
-      const bool live = rr < p.rows;
-      float t[V][8];
+      const bool live = row + u * step < p.rows;
       float s1 = 0.f, s2 = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float g[8];
-        cvt8<DT>(rg[u][j], g);
-        if (gate_z) {
-          float z[8];
-          cvt8<DT>(rz[u][j], z);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) g[k] *= z[k] > 0.f ? 1.f : p.slope;
+        for (int k = 0; k < 8; ++k) x[u][j][k] = (x[u][j][k] - mean[u]) * inv[u];
+        if (gate_x) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            t[u][j][k] *= ln_affine(x[u][j][k], ga[j][k], k < nv[j] ? p.beta[c[j] + k] : 0.f) > 0.f ? 1.f : p.slope;
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float h = (x[u][j][k] - mean[u]) * inv[u];
-          if (gate_x) g[k] *= ln_affine(h, ga[j][k], k < nv[j] ? p.beta[c[j] + k] : 0.f) > 0.f ? 1.f : p.slope;
           const bool ok = k < nv[j] && live;
-          const float hk = ok ? h : 0.f, gk = ok ? g[k] : 0.f;
-          x[u][j][k] = hk;
-          dg[j][k] += gk * hk;
-          db[j][k] += gk;
-          t[j][k] = gk * ga[j][k];
-          s1 += t[j][k];
-          s2 += t[j][k] * hk;
+          const float h = ok ? x[u][j][k] : 0.f, g = ok ? t[u][j][k] : 0.f;
+          x[u][j][k] = h;
+          dg[j][k] = __builtin_fmaf(g, h, dg[j][k]);
+          db[j][k] += g;
+          t[u][j][k] = g * ga[j][k];
+          s1 += t[u][j][k];
+          s2 = __builtin_fmaf(t[u][j][k], h, s2);
         }
       }
-      s1 = row_sum<WG>(s1, p.group, red) * rc;
-      s2 = row_sum<WG>(s2, p.group, red) * rc;
-      if (p.out && live) {
+      s[2 * u] = s1; s[2 * u + 1] = s2;
+    }
+    row_sums<WG, 2 * U>(s, p.group, red, turn);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          if (c[j] >= p.C) continue;
-          float o[8];
+    for (int u = 0; u < U; ++u) {
+      const long long rr = row + u * step;
+      if (!p.out || rr >= p.rows) continue;
+      const float s1 = s[2 * u] * rc, s2 = s[2 * u + 1] * rc;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) o[k] = k < nv[j] ? inv[u] * (t[j][k] - s1 - x[u][j][k] * s2) : 0.f;
-          st8<DT>(p.out, rr * p.ops + c[j], o);
-        }
+      for (int j = 0; j < V; ++j) {
+        if (c[j] >= p.C) continue;
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = k < nv[j] ? inv[u] * (t[u][j][k] - s1 - x[u][j][k] * s2) : 0.f;
+        st8<DT>(p.out, rr * p.ops + c[j], o);
       }
     }
   }
@@ -275,7 +296,6 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         for (int o = p.group; o < 64; o <<= 1) { dg[j][k] += __shfl_xor(dg[j][k], o); db[j][k] += __shfl_xor(db[j][k], o); }
-    float* part = lds + 4;
     const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63, span = p.group * V * 8;
     for (int w = 0; w < 4; ++w) {
       if (wid == w && lane < p.group) {
@@ -283,27 +303,26 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
         for (int j = 0; j < V; ++j)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            part[c[j] + k] = (w ? part[c[j] + k] : 0.f) + dg[j][k];
-            part[span + c[j] + k] = (w ? part[span + c[j] + k] : 0.f) + db[j][k];
+            lds[c[j] + k] = (w ? lds[c[j] + k] : 0.f) + dg[j][k];
+            lds[span + c[j] + k] = (w ? lds[span + c[j] + k] : 0.f) + db[j][k];
           }
       }
       __syncthreads();
     }
-    for (int i = threadIdx.x; i < 2 * p.C_real; i += 256) prow[i] = part[i < p.C_real ? i : span + i - p.C_real];
+    for (int i = threadIdx.x; i < 2 * p.C_real; i += 256) prow[i] = lds[i < p.C_real ? i : span + i - p.C_real];
   }
 }
 
 #define LN_MAX_C 8192
 struct LNShape { bool wg; int group, v; };
-// lanes and vectors of a row of C channels: one vector a lane up to a wave's width, then two and four, then a workgroup
+// Lanes and vectors of a row of C channels: up to a wave of one vector a lane, then two; from there on a workgroup, of one,
+// two and four (four vectors a lane of a wave would keep the backward to one wave a SIMD).
 static LNShape ln_shape(int C) {
   const int c8 = C / 8;
   LNShape s = {false, 4, 1};                 // four lanes at least: a block of the 8-bit form is four lanes wide
   while (s.group < c8 && s.group < 64) s.group *= 2;
-  while (s.group * s.v < c8 && s.v < 4) s.v *= 2;
-  if (s.group * s.v < c8) {
-    s.wg = true; s.group = 256; s.v = c8 <= 512 ? 2 : 4;
-  }
+  if (c8 > 64) s.v = 2;
+  if (c8 > 128) { s.wg = true; s.group = 256; s.v = c8 <= 256 ? 1 : (c8 <= 512 ? 2 : 4); }
   return s;
 }
 static bool ln_args_ok(int dtype, long long npix, int C, int C_real) {
@@ -317,18 +336,24 @@ static long long ln_blocks(long long npix, const LNShape& s, int unroll) {
   return (npix + per - 1) / per;
 }
 
+// Rows a lane works on at once (beside those it has under way), and workgroups: about what the registers let reside, which
+// then walk the rows.  More of either costs: at 32768 pixels of 1024 bf16 channels kept in 8 bits, forward and backward
+// take 41 and 37 us with these, 48 and 47 with 1536 and 1280 workgroups, 54 and 56 with 2048 and 1024 that fetch no row
+// ahead.
+static int ln_unroll(const LNShape& s) { return s.v == 1 ? 2 : 1; }
+#define LN_FWD_BLOCKS 1024
+#define LN_BWD_BLOCKS 768
+
 template <int DT, bool KEEP> static int ln_fwd_launch(const LNParams& p, const LNShape& s, hipStream_t st) {
-  // rows in flight per lane: four of one vector, two of two, else one
-  const int U = s.wg ? 1 : (s.v == 1 ? 4 : (s.v == 2 ? 2 : 1));
-  long long blocks = ln_blocks(p.rows, s, U);
-  if (blocks > 2048) blocks = 2048;
+  long long blocks = ln_blocks(p.rows, s, ln_unroll(s));
+  if (blocks > LN_FWD_BLOCKS) blocks = LN_FWD_BLOCKS;
   const dim3 g((unsigned)blocks), b(256);
   if (s.wg) {
-    if (s.v == 2) hipLaunchKernelGGL((ln_fwd_kernel<DT, true, 2, 1, KEEP>), g, b, 0, st, p);
+    if (s.v == 1) hipLaunchKernelGGL((ln_fwd_kernel<DT, true, 1, 2, KEEP>), g, b, 0, st, p);
+    else if (s.v == 2) hipLaunchKernelGGL((ln_fwd_kernel<DT, true, 2, 1, KEEP>), g, b, 0, st, p);
     else hipLaunchKernelGGL((ln_fwd_kernel<DT, true, 4, 1, KEEP>), g, b, 0, st, p);
-  } else if (s.v == 1) hipLaunchKernelGGL((ln_fwd_kernel<DT, false, 1, 4, KEEP>), g, b, 0, st, p);
-  else if (s.v == 2) hipLaunchKernelGGL((ln_fwd_kernel<DT, false, 2, 2, KEEP>), g, b, 0, st, p);
-  else hipLaunchKernelGGL((ln_fwd_kernel<DT, false, 4, 1, KEEP>), g, b, 0, st, p);
+  } else if (s.v == 1) hipLaunchKernelGGL((ln_fwd_kernel<DT, false, 1, 2, KEEP>), g, b, 0, st, p);
+  else hipLaunchKernelGGL((ln_fwd_kernel<DT, false, 2, 1, KEEP>), g, b, 0, st, p);
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }
@@ -356,23 +381,22 @@ extern "C" int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z,
   return q8 ? ln_fwd_launch<CSMRI_BF16, true>(p, s, st) : ln_fwd_launch<CSMRI_BF16, false>(p, s, st);
 }
 
-static int ln_bwd_unroll(const LNShape& s) { return !s.wg && s.v == 1 ? 2 : 1; }
 extern "C" int csmri_ln_bwd_rows(long long npix, int C) {
   if (npix <= 0 || C <= 0) return 0;
   const LNShape s = ln_shape(C);
-  const long long b = ln_blocks(npix, s, ln_bwd_unroll(s));
-  return (int)(b > 1024 ? 1024 : b);
+  const long long b = ln_blocks(npix, s, ln_unroll(s));
+  return (int)(b > LN_BWD_BLOCKS ? LN_BWD_BLOCKS : b);
 }
 
 template <int DT, bool KEPT> static int ln_bwd_launch(const LNParams& p, const LNShape& s, int blocks, hipStream_t st) {
   const dim3 g(blocks), b(256);
-  const size_t lds = (4 + (s.wg ? 0 : 2 * (size_t)s.group * s.v * 8)) * sizeof(float);
+  const size_t lds = s.wg ? 0 : 2 * (size_t)s.group * s.v * 8 * sizeof(float);
   if (s.wg) {
-    if (s.v == 2) hipLaunchKernelGGL((ln_bwd_kernel<DT, true, 2, 1, KEPT>), g, b, lds, st, p);
+    if (s.v == 1) hipLaunchKernelGGL((ln_bwd_kernel<DT, true, 1, 2, KEPT>), g, b, lds, st, p);
+    else if (s.v == 2) hipLaunchKernelGGL((ln_bwd_kernel<DT, true, 2, 1, KEPT>), g, b, lds, st, p);
     else hipLaunchKernelGGL((ln_bwd_kernel<DT, true, 4, 1, KEPT>), g, b, lds, st, p);
   } else if (s.v == 1) hipLaunchKernelGGL((ln_bwd_kernel<DT, false, 1, 2, KEPT>), g, b, lds, st, p);
-  else if (s.v == 2) hipLaunchKernelGGL((ln_bwd_kernel<DT, false, 2, 1, KEPT>), g, b, lds, st, p);
-  else hipLaunchKernelGGL((ln_bwd_kernel<DT, false, 4, 1, KEPT>), g, b, lds, st, p);
+  else hipLaunchKernelGGL((ln_bwd_kernel<DT, false, 2, 1, KEPT>), g, b, lds, st, p);
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }

@@ -24,14 +24,53 @@ __device__ __forceinline__ int micro_exp(unsigned amax) {
   return e < MICRO_MIN_EXP ? MICRO_MIN_EXP : e;
 }
 
+// Values of neighbouring lanes through the data-parallel paths of the vector unit (a shuffle through LDS takes ten times as
+// long): lane ^ 1, lane ^ 2, and the mirror images inside 8 and 16 lanes, which stand for lane ^ 4 and lane ^ 8 once the
+// lanes of a quad (of an eighth) agree.
+#define DPP_XOR1 0xB1
+#define DPP_XOR2 0x4E
+#define DPP_MIRROR8 0x141
+#define DPP_MIRROR16 0x140
+template <int CTRL> __device__ __forceinline__ unsigned dpp_u(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL> __device__ __forceinline__ float dpp_f(float v) { return __uint_as_float(dpp_u<CTRL>(__float_as_uint(v))); }
+
+// sums over aligned groups of `group` lanes (4 .. 64, a power of two), the same bits in every lane of a group
+template <int N> __device__ __forceinline__ void group_sums(float (&v)[N], int group) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += dpp_f<DPP_XOR1>(v[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += dpp_f<DPP_XOR2>(v[i]);
+  if (group < 8) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += dpp_f<DPP_MIRROR8>(v[i]);
+  if (group < 16) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] += dpp_f<DPP_MIRROR16>(v[i]);
+  if (group < 32) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (group < 64) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+}
+
 // eight channels per lane, four consecutive lanes per block: the block's largest magnitude in each of them
 __device__ __forceinline__ unsigned block_amax(const float* v) {
   unsigned m = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) { const unsigned a = abs_bits(v[k]); m = a > m ? a : m; }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) { const unsigned t = __shfl_xor(m, o); m = t > m ? t : m; }
-  return m;
+  unsigned t = dpp_u<DPP_XOR1>(m);
+  m = t > m ? t : m;
+  t = dpp_u<DPP_XOR2>(m);
+  return t > m ? t : m;
 }
 
 // eight values -> eight e4m3 codes and their scale byte
