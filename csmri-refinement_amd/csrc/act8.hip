@@ -206,15 +206,20 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
 // pending one; a second set of registers, to load two steps ahead, costs more in occupancy than it hides.)  Bound by the
 // matrix unit and the steps around it: of the 192 us at 2048 x 2048 channels and 16384 pixels, a loop of the products,
 // barriers and stores alone takes 132.
-template <int DT, int FN, int FC, int WN, int WC, int KP>
-__global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WParams p) {
+//
+// GK = 2: a second set of waves takes every other step, with stages of its own, and hands its sums over at the end -- the
+// occupancy of two workgroups with the partial sums of one, which otherwise cost as much as the small layers' operands.
+template <int DT, int FN, int FC, int WN, int WC, int KP, int GK>
+__global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const A8WParams p) {
   constexpr int NW = WN * WC, NT = 64 * NW, BN = 16 * FN * WN, BC = 16 * FC * WC, CN = BN / 8, CC = BC / 8;
   constexpr int PL = DT == CSMRI_F32 ? 3 : 1, ES = DT == CSMRI_F32 ? 4 : 2;
   constexpr int YIMG = KP * BN * 2, XIMG = KP * BC * 2, STG = PL * YIMG + XIMG;
   constexpr int NY = KP * CN / NT, NX = KP * CC / NT;            // chunks of eight channels a thread and stage
   static_assert(KP * CN % NT == 0 && KP * CC % NT == 0, "whole chunks per thread");
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid / WC, wc = wid % WC;
+  const int tid = threadIdx.x % NT, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid / WC, wc = wid % WC;
+  const int part = __builtin_amdgcn_readfirstlane(threadIdx.x / NT);
+  char* stages = smem + part * 2 * STG;
   const int tiles = p.ntiles * p.ctiles;
   // an XCD takes neighbouring tiles of the same pixels, which then meet in its L2
   const int wg = xcd_remap(blockIdx.x, tiles * p.splits), split = wg / tiles, tile = wg - split * tiles;
@@ -222,7 +227,7 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
   const int n0 = nt * BN, c0 = ct * BC;
   const long long pb = split * p.chunk, pe = pb + p.chunk < p.npix ? pb + p.chunk : p.npix;
   const int sblocks = (p.Cin + MICRO_BLOCK - 1) / MICRO_BLOCK;
-  const int steps = pe > pb ? (int)((pe - pb + KP - 1) / KP) : 0;
+  const int steps = pe > pb ? (int)((pe - pb + KP - 1) / KP) : 0, mine = (steps + GK - 1) / GK;   // step s of a part: GK s + part
 
   constexpr int NB = FN / WC;                                     // fragments whose column sums a wave takes
   static_assert(FN % WC == 0, "every wave of a row takes as many");
@@ -250,9 +255,9 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
   }
   raw8<DT> yv[2][NY]; u32x2_t xv[2][NX]; unsigned sv[2][NX];
   auto left_of = [&](int k) { const long long l = pe - pb - (long long)k * KP; return l < KP ? (int)l : KP; };
-  // (behind the last step: the last one again, not used)
-  auto fetch = [&](int k, int b) {
-    k = min(k, steps - 1);
+  // (behind the last step: the last one again, with a dY of zero)
+  auto fetch = [&](int s, int b) {
+    const int k = min(s * GK + part, steps - 1);
     const long long pix = pb + (long long)k * KP;
     const char* yb = p.dy + pix * p.dyps * ES;
     const unsigned char* xb = p.q + pix * p.Cin; const unsigned char* sb = p.s + pix * sblocks;
@@ -266,9 +271,9 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
       sv[b][j] = sb[(unsigned)(r * sblocks + (xch[j] >> 5))];
     }
   };
-  auto place = [&](int k, int b) {
-    char* yi = smem + (k & 1) * STG; char* xi = yi + PL * YIMG;
-    const int left = left_of(k);
+  auto place = [&](int s, int b) {
+    char* yi = stages + (s & 1) * STG; char* xi = yi + PL * YIMG;
+    const int left = left_of(s * GK + part);
     if (left < KP) {
 #pragma unroll
       for (int j = 0; j < NY; ++j)
@@ -311,8 +316,8 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
   const bf16x8_t ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
   const bool want_b = p.db && ct == 0;
   auto run = [&](auto with_bias) {
-    auto multiply = [&](int k) {
-      const char* yi = smem + (k & 1) * STG; const char* xi = yi + PL * YIMG;
+    auto multiply = [&](int s) {
+      const char* yi = stages + (s & 1) * STG; const char* xi = yi + PL * YIMG;
 #pragma unroll
       for (int kk = 0; kk < KP; kk += 32) {
         bf16x8_t xf[FC];
@@ -342,16 +347,37 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
     fetch(0, 0);
     place(0, 0);
     fetch(1, 0);
-    for (int k = 0; k < steps; ++k) {
-      barrier();                                  // stage k is there for everyone; everyone has read stage k - 1
-      place(k + 1, 0);
-      fetch(k + 2, 0);
+    for (int s = 0; s < mine; ++s) {
+      barrier();                                  // stage s is there for everyone; everyone has read stage s - 1
+      place(s + 1, 0);
+      fetch(s + 2, 0);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(k);
+      multiply(s);
     }
   };
   if (want_b) run(std::true_type{});
   else run(std::false_type{});
+  if constexpr (GK == 2) {
+    static_assert((FN * FC + NB) * NT * 16 <= 4 * STG, "the sums handed over share the stages' place");
+    f32x4_t* sums = (f32x4_t*)smem + tid;
+    barrier();
+    if (part == 1) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FC; ++j) sums[(i * FC + j) * NT] = acc[i][j];
+#pragma unroll
+      for (int i = 0; i < NB; ++i) sums[(FN * FC + i) * NT] = accb[i];
+    }
+    barrier();
+    if (part == 1) return;
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FC; ++j) acc[i][j] += sums[(i * FC + j) * NT];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) accb[i] += sums[(FN * FC + i) * NT];
+  }
   // lane l holds rows n = 4 g + r, column c = l & 15 of each fragment
   const long long len = (long long)p.Cout_real * p.Cin_real;
   float* dw = p.splits > 1 ? p.slab + split * (len + p.Cout_real) : p.dw;
@@ -383,7 +409,7 @@ __global__ __launch_bounds__(64 * WN * WC, 2) void act8_wgrad_kernel(const A8WPa
   }
 }
 
-// Tile: 64 or 128 a side by the channel counts, two workgroups a CU; 256 x 256 (an fp32 dY's three planes do not fit it),
+// Tile: 64 or 128 a side by the channel counts; 256 x 256 (an fp32 dY's three planes do not fit it),
 // which reads LDS a third less per product, where 2048 pixels a split still leave three quarters of the CUs a workgroup.
 // 2048 x 2048 channels, 16384 pixels: 192 us against 225 with 128 x 128; 512 x 512, 8192 pixels: 46 against 35.
 struct A8WTile { int bn, bc; };
@@ -396,25 +422,25 @@ extern "C" int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, i
   if (npix <= 0 || Cout <= 0 || Cin <= 0) return 1;
   const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
   const long long tiles = (long long)cdiv(Cout, t.bn) * cdiv(Cin, t.bc);
-  long long s = (t.bn == 256 ? 256 : 512) / tiles;
-  const long long most = npix / 512;                          // at least eight or sixteen steps each
+  long long s = 256 / tiles;                                  // one workgroup of eight waves a CU
+  const long long most = npix / 512;                          // at least eight steps each
   if (s > most) s = most;
   return s < 1 ? 1 : (int)s;
 }
-template <int DT, int FN, int FC, int WN, int WC, int KP> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
-  constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = 2 * KP * 2 * (BN * (DT == CSMRI_F32 ? 3 : 1) + BC);
-  auto kern = act8_wgrad_kernel<DT, FN, FC, WN, WC, KP>;
+template <int DT, int FN, int FC, int WN, int WC, int KP, int GK> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
+  constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = GK * 2 * KP * 2 * (BN * (DT == CSMRI_F32 ? 3 : 1) + BC);
+  auto kern = act8_wgrad_kernel<DT, FN, FC, WN, WC, KP, GK>;
   CSMRI_SET_MAX_LDS(kern, LDS);
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WN * WC), LDS, st, p);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * WN * WC * GK), LDS, st, p);
   CSMRI_LAUNCH_CHECK();
   return CSMRI_OK;
 }
-// pixels a step: 64, for fewer barriers, where two stages of that fit two workgroups into a CU's LDS
+// pixels a step: 64, for fewer barriers, where two stages of that fit LDS twice
 template <int DT> static int a8w_dispatch(const A8WTile& t, const A8WParams& p, unsigned grid, hipStream_t st) {
   constexpr int KP = DT == CSMRI_F32 ? 32 : 64;
-  if constexpr (DT == CSMRI_BF16) if (t.bn == 256) return a8w_launch<DT, 8, 4, 2, 4, 32>(p, grid, st);
-  if (t.bn == 128) return t.bc == 128 ? a8w_launch<DT, 4, 4, 2, 2, KP>(p, grid, st) : a8w_launch<DT, 4, 2, 2, 2, KP>(p, grid, st);
-  return t.bc == 128 ? a8w_launch<DT, 2, 4, 2, 2, KP>(p, grid, st) : a8w_launch<DT, 2, 2, 2, 2, KP>(p, grid, st);
+  if constexpr (DT == CSMRI_BF16) if (t.bn == 256) return a8w_launch<DT, 8, 4, 2, 4, 32, 1>(p, grid, st);
+  if (t.bn == 128) return t.bc == 128 ? a8w_launch<DT, 4, 4, 2, 2, KP, 2>(p, grid, st) : a8w_launch<DT, 4, 2, 2, 2, KP, 2>(p, grid, st);
+  return t.bc == 128 ? a8w_launch<DT, 2, 4, 2, 2, KP, 2>(p, grid, st) : a8w_launch<DT, 2, 2, 2, 2, KP, 2>(p, grid, st);
 }
 extern "C" size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real) {
   return splits > 1 ? (size_t)splits * ((size_t)Cout_real * Cin_real + Cout_real) * sizeof(float) : 0;
