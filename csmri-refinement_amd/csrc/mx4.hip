@@ -25,6 +25,48 @@ __device__ __forceinline__ unsigned mx4_pack8(const float* v, float scale) {
   q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[6], v[7], scale, 3);
   return q;
 }
+// A lane's whole block, 32 consecutive channels -> 16 bytes of codes and the scale byte.  bf16 stays packed: its magnitudes
+// order as 16-bit integers, and the conversion takes pairs.
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2_t;
+template <int DT> __device__ __forceinline__ u32x4_t mx4_pack_block(const raw8<DT> (&raw)[4], int& scale) {
+  unsigned amax;
+  if constexpr (DT == CSMRI_BF16) {
+    u16x2_t m = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, raw[i].a[k] & 0x7fff7fffu));
+    amax = (unsigned)(m[0] > m[1] ? m[0] : m[1]) << 16;
+  } else {
+    amax = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) { amax = max(amax, abs_bits(raw[i].a[k])); amax = max(amax, abs_bits(raw[i].b[k])); }
+  }
+  const bool fin = micro_finite(amax);
+  const int e = fin ? micro_exp(amax) - 2 : 0;
+  const float s = exp2i(e);
+  u32x4_t q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == CSMRI_BF16) {
+      // (named words: a bit cast of a vector's element takes the vector's first)
+      const unsigned w0 = raw[i].a[0], w1 = raw[i].a[1], w2 = raw[i].a[2], w3 = raw[i].a[3];
+      unsigned t = 0;
+      t = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(t, __builtin_bit_cast(bf16x2_t, w0), s, 0);
+      t = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(t, __builtin_bit_cast(bf16x2_t, w1), s, 1);
+      t = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(t, __builtin_bit_cast(bf16x2_t, w2), s, 2);
+      q[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(t, __builtin_bit_cast(bf16x2_t, w3), s, 3);
+    } else {
+      float v[8];
+      cvt8<DT>(raw[i], v);
+      q[i] = mx4_pack8(v, s);
+    }
+  }
+  scale = fin ? e + 127 : MICRO_NAN;
+  return q;
+}
 __device__ __forceinline__ i32x8_t mx4_operand(u32x4_t c) {
   return (i32x8_t){(int)c[0], (int)c[1], (int)c[2], (int)c[3], 0, 0, 0, 0};
 }
@@ -209,22 +251,7 @@ __global__ __launch_bounds__(512) void mx4_skinny_kernel(const MxParams p) {
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int f = 0; f < MF; ++f) {
-        if constexpr (QX >= 0) {
-          float v[4][8];
-          unsigned amax = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            cvt8<QX>(raw[u][f][i], v[i]);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) { const unsigned a = abs_bits(v[i][q]); amax = a > amax ? a : amax; }
-          }
-          const int e = micro_exp(amax) - 2;
-          const bool fin = micro_finite(amax);
-          const float s = exp2i(fin ? e : 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) xc[u][f][i] = mx4_pack8(v[i], s);
-          xsc[u][f] = fin ? e + 127 : MICRO_NAN;
-        }
+        if constexpr (QX >= 0) xc[u][f] = mx4_pack_block<QX>(raw[u][f], xsc[u][f]);
         acc[f] = mx4_mfma(mx4_operand(wc[u]), wsc[u], mx4_operand(xc[u][f]), xsc[u][f], acc[f]);
       }
   }
@@ -414,10 +441,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); \
         barrier(); \
       } \
-      __builtin_amdgcn_s_setprio(1); \
       MX_MUL(2 * U) \
       MX_MUL(2 * U + 1) \
-      __builtin_amdgcn_s_setprio(0); \
       if (U == 1 && !(PP && late)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
       if (PP || U == 1) barrier(); \
       if (k + U + 1 >= K) break; \
