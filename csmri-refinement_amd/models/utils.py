@@ -47,6 +47,29 @@ def set_fp8_forward(module, on=True):
   return n
 
 
+def _set_layer_flag(module, name, on, wanted):
+  n = 0
+  for m in module.modules():
+    if isinstance(m, ConvParams):
+      setattr(m, name, bool(on))
+      if m.layer is not None and not m.layer.frozen and wanted(m.layer):
+        setattr(m.layer, name, bool(on))
+        n += 1
+  return n
+
+
+def set_mx4_forward(module, on=True):
+  """Switch the 4-bit forward products of every trainable 1 x 1 convolution under ``module`` (ops.ConvLayer.mx4); returns
+  how many layers that concerns.  Gradients are those of the 16- or 32-bit path, through the rounding."""
+  return _set_layer_flag(module, 'mx4', on, lambda layer: layer.pointwise())
+
+
+def set_keep8(module, on=True):
+  """Keep the inputs of every trainable convolution under ``module`` in 8 bits for their weight gradients
+  (ops.ConvLayer.keep8); returns how many layers that concerns.  Outputs and data gradients do not change."""
+  return _set_layer_flag(module, 'keep8', on, lambda layer: True)
+
+
 def default_compute_dtype():
   return _DEFAULT_DTYPE[0]
 
@@ -92,6 +115,8 @@ class ConvParams(nn.Module):
                                upsample=upsample, frozen=frozen)
     self._layer_args = (stride, pads, border, dtype, upsample, frozen)
     self.layer.fp8 = bool(getattr(self, 'fp8', _FP8_FORWARD[0] and FP8_TRAINABLE)) and not frozen
+    self.layer.mx4 = bool(getattr(self, 'mx4', False)) and not frozen
+    self.layer.keep8 = bool(getattr(self, 'keep8', False)) and not frozen
     return self.layer
 
   def _apply(self, fn, *a, **k):

@@ -515,6 +515,48 @@ def test_block_of_norm_and_4bit_product_trains(ops):
 
 
 @pytest.mark.gpu
+def test_unet_with_kept_activations(ops):
+  """set_keep8 / set_mx4_forward on a U-Net: the kept inputs change no output, no data gradient and no BatchNorm gradient;
+  the forward pass leaves less memory behind.  The 4-bit product reaches the 1 x 1 head alone."""
+  from models import unet, utils
+
+  def build():
+    torch.manual_seed(3)
+    return unet.UNET(1, 1, 2, [32, 64], [32], 'none', kernel_size=3, upsampling_mode='nn-resize-conv', padding='reflection',
+                     decoder_act_upsampling_only=True, compute_dtype='bf16').cuda().train()
+
+  g = torch.Generator().manual_seed(4)
+  x0, gy = torch.randn(2, 1, 64, 64, generator=g).cuda(), torch.randn(2, 1, 64, 64, generator=g).cuda()
+  res = []
+  for keep in (False, True):
+    net = build()
+    if keep:
+      assert utils.set_keep8(net) == 8 and utils.set_keep8(net.cuda()) == 8
+    x = x0.clone().requires_grad_(True)
+    before = torch.cuda.memory_allocated()
+    y = net(x)
+    held = torch.cuda.memory_allocated() - before
+    y.backward(gy)
+    res.append((y.detach(), x.grad, held, {n: p.grad for n, p in net.named_parameters()}))
+  assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
+  assert res[1][2] < 0.9 * res[0][2], (res[0][2], res[1][2])
+  for n, p in res[0][3].items():
+    if p.dim() == 1 and 'head' not in n:
+      assert torch.equal(p, res[1][3][n]), n
+    else:
+      assert torch.isfinite(res[1][3][n]).all() and res[1][3][n].any(), n
+  net = build()
+  assert utils.set_mx4_forward(net) == 1 and net.head['0'].layer.mx4
+  y = net(x0)
+  d = (y.detach() - res[0][0]).abs()
+  assert d.any() and torch.isfinite(y).all()
+  y.backward(gy)
+  assert net.head['0'].weight.grad.any()
+  utils.set_mx4_forward(net, False)
+  assert torch.equal(build()(x0), res[0][0])
+
+
+@pytest.mark.gpu
 def test_captured_step_replays_like_the_eager_one(ops):
   dt = torch.bfloat16
   layer = conv_layer(ops, 64, 64, 1, dt, (0, 0, 0, 0), 31)
