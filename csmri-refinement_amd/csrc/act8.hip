@@ -349,10 +349,12 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
     fetch(1, 0);
     for (int s = 0; s < mine; ++s) {
       barrier();                                  // stage s is there for everyone; everyone has read stage s - 1
+      // half of the waves multiply first, so that staging and products run side by side
+      if (wn & 1) { multiply(s); __builtin_amdgcn_sched_barrier(0); }
       place(s + 1, 0);
       fetch(s + 2, 0);
       __builtin_amdgcn_sched_barrier(0);
-      multiply(s);
+      if (!(wn & 1)) multiply(s);
     }
   };
   if (want_b) run(std::true_type{});
