@@ -144,8 +144,9 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const unsigned* __r
   }
 }
 
+#define MX4_MAX_K (1 << 24)    // channels of a row: a tile's 256 rows of codes and scales stay within 32-bit offsets
 static bool mx4_shape_ok(long long rows, int K, int ps, int dtype) {
-  return rows >= 0 && K > 0 && K % 8 == 0 && ps >= K && (dtype == CSMRI_F32 || dtype == CSMRI_BF16);
+  return rows >= 0 && K > 0 && K % 8 == 0 && K <= MX4_MAX_K && ps >= K && (dtype == CSMRI_F32 || dtype == CSMRI_BF16);
 }
 static bool mx4_rows_aligned(const void* p, int ps, int dtype) {
   return ((uintptr_t)p & 15) == 0 && ((long long)ps * dtype_size(dtype)) % 16 == 0;
@@ -326,7 +327,7 @@ __device__ __forceinline__ void mx4_epilogue(const MxParams& p, long long m0, in
   }
 }
 
-template <int FM, int FN, int WM, int WN, int OCC, bool PP>
+template <int FM, int FN, int WM, int WN, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxParams p) {
   constexpr int NW = WM * WN, BM = 32 * FM * WM, BN = 32 * FN * WN, STG = (BM + BN) * 128, SCL = (BM + BN) * 16;
   constexpr int NA = BM / (8 * NW), NB = BN / (8 * NW), NS = ((BM + BN) / 64 + NW - 1) / NW;
@@ -337,7 +338,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
   const int wm = wid / WN, wn = wid % WN, r32 = lane & 31, h = lane >> 5;
   const int tz = xcd_remap(blockIdx.x, p.mtiles * p.ntiles * p.splits), split = tz / (p.mtiles * p.ntiles);
   const int t = tz - split * p.mtiles * p.ntiles;
-  const int mt = t / p.ntiles, nt = t - mt * p.ntiles, k0 = split * p.schunk;
+  // bands of eight row tiles: what runs on an XCD at one time is about square and shares its operands in L2
+  // (8192^3: 309 us, 318 in row order; 16384 x 4096 x 4096: 186, 192; smaller ones alike)
+  const int band = t / (8 * p.ntiles), r = t - band * 8 * p.ntiles, bm = min(8, p.mtiles - band * 8);
+  const int mt = band * 8 + r % bm, nt = r / bm, k0 = split * p.schunk;
   const long long m0 = (long long)mt * BM; const int n0 = nt * BN;
   const int mrows = p.M - m0 < BM ? (int)(p.M - m0) : BM, nrows = p.N - n0 < BN ? p.N - n0 : BN;
   const char* xb = p.xq + m0 * p.cb + k0 * 64; const char* wb = p.wq + (long long)n0 * p.cb + k0 * 64;
@@ -425,26 +429,20 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  const bool late = PP && wm >= WM / 2;
   issue(0);
   for (int i = tid; i < BN; i += 64 * NW) sbias[i] = p.bias && p.splits == 1 && n0 + i < p.N ? p.bias[n0 + i] : 0.f;
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   barrier();
-  if (late) barrier();
-  // PP: the two halves of the workgroup alternate, one reads its fragments while the other one multiplies
 #define MX_STEP(U) \
     { \
       if (U == 0 && k + 2 < K) issue((k >> 1) + 1); \
       load(k + U); \
-      if (PP) { \
-        if (U == 1 && late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); \
-        barrier(); \
-      } \
       MX_MUL(2 * U) \
       MX_MUL(2 * U + 1) \
-      if (U == 1 && !(PP && late)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
-      if (PP || U == 1) barrier(); \
+      if (U == 1) { \
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); \
+        barrier(); \
+      } \
       if (k + U + 1 >= K) break; \
     }
   for (int k = 0;; k += 2) {
@@ -453,8 +451,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
   }
 #undef MX_STEP
 #undef MX_MUL
-  if (PP && !late) barrier();
-  if (!PP) barrier();
+  barrier();
   char* img = smem + wid * FM * 4096;
   if (p.splits > 1) {
     MxParams q = p;                                        // a partial sum: no bias, no activation
@@ -463,10 +460,10 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
   } else if (p.out_dt == CSMRI_BF16) mx4_epilogue<CSMRI_BF16, FM, FN>(p, m0 + wm * FM * 32, n0 + wn * FN * 32, acc, img, sbias + wn * FN * 32, lane);
   else mx4_epilogue<CSMRI_F32, FM, FN>(p, m0 + wm * FM * 32, n0 + wn * FN * 32, acc, img, sbias + wn * FN * 32, lane);
 }
-template <int FM, int FN, int WM, int WN, int OCC, bool PP> static int mx4_gemm_launch(MxParams& p, hipStream_t st) {
+template <int FM, int FN, int WM, int WN, int OCC> static int mx4_gemm_launch(MxParams& p, hipStream_t st) {
   constexpr int BM = 32 * FM * WM, BN = 32 * FN * WN, LDS = 2 * (BM + BN) * 128 + 2 * (BM + BN) * 16 + BN * 4;
   static_assert(WM * WN * FM * 4096 <= 2 * (BM + BN) * 128, "the output images share the stages' place");
-  auto kern = mx4_gemm_kernel<FM, FN, WM, WN, OCC, PP>;
+  auto kern = mx4_gemm_kernel<FM, FN, WM, WN, OCC>;
   const long long mt = (p.M + BM - 1) / BM, nt = (p.N + BN - 1) / BN;
   if (mt * nt * p.splits > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
   p.mtiles = (int)mt; p.ntiles = (int)nt;
@@ -489,31 +486,53 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const MxParams p) {
   }
 }
 
-#define MX4_QUANT_ROWS 16      // up to here the product quantises x itself
-#define MX4_SKINNY_ROWS 64     // up to here its rows fit the fragments of one wave
-// Splits of the channels for the tiled kernel: where its 128 x 128 tiles are few and the channels many, until there is a
-// workgroup for each CU; every split keeps 512 channels or more.
+// Few rows: up to 64, whose fragments fit one wave, as long as the workgroups of 16 outputs make no more than 1024 sets of
+// 16 rows -- each of them reads all of x.  Rows x K x outputs, us here and with the tiles: 64 x 4096 x 4096 11 / 13,
+// 33 x 4096 x 4096 8 / 11, 32 x 4096 x 8192 13 / 15, 16 x 1024 x 16384 6.1 / 6.5; beyond 64 x 4096 x 8192 20 / 15,
+// 32 x 1024 x 16384 9.2 / 6.6.
+static bool mx4_few(long long rows, int N) { return rows <= 64 && (rows + 15) / 16 * ((N + 15LL) / 16) <= 1024; }
+// Of these up to 16 rows are quantised in the product itself, by every workgroup again: with 512 workgroups or fewer that
+// takes less than a launch and a pass of its own (4 x 4096 x 4096: 6.0, 7.2 us; 8 x 4096 x 8192: 10.6, 10.3;
+// 4 x 4096 x 16384: 17.0, 15.0).
+static bool mx4_packs(long long rows, int N) { return rows <= 16 && N <= 8192; }
+// Splits of the channels for the tiled kernel, where its 128 x 128 tiles leave CUs without one.  A group of 512 channels
+// takes a workgroup 1.4 us; joining takes 3.5 us and 0.5 us for each MiB of partial sums (512 x 2048 x 1024 in one part
+// 9.3 us, in four 12.3; 512 x 8192 x 2048 26 and 21; 128 x 16384 x 4096 in eight parts 18, in one 49): the least
+// sum of these, in quarters of a group.
 static int mx4_splits(long long rows, int K, int N) {
-  if (rows <= MX4_SKINNY_ROWS) return 1;
-  const long long tiles = ((rows + 127) / 128) * ((N + 127) / 128);
-  const int groups = (K + 511) / 512;
-  if (tiles > 64 || groups < 4) return 1;
-  const int want = (int)(256 / tiles), s = want < groups ? want : groups, per = (groups + s - 1) / s;
-  return (groups + per - 1) / per;
+  if (mx4_few(rows, N)) return 1;
+  const long long tiles = ((rows + 127) / 128) * ((N + 127LL) / 128), npad = (N + 7LL) / 8 * 8;
+  const int groups = (int)((K + 511LL) / 512);
+  if (tiles > 128) return 1;
+  const int most = (int)(256 / tiles) < groups ? (int)(256 / tiles) : groups;
+  int best = 1; long long least = 4LL * groups;
+  for (int s = 2; s <= most; ++s) {
+    const int per = (groups + s - 1) / s, n = (groups + per - 1) / per;
+    const long long cost = 4LL * per + 10 + ((6 * n * rows * npad) >> 20);
+    if (cost < least) { least = cost; best = n; }
+  }
+  return best;
 }
-static size_t mx4_quant_bytes(int x_dtype, long long rows, int K) {
-  return x_dtype == CSMRI_MX4 || rows <= MX4_QUANT_ROWS ? 0 : (size_t)rows * (mx4_code_bytes(K) + mx4_scale_bytes(K));
+// The 256 x 256 tile reads each operand half as often and has a CU to itself.  It is taken where there are more 128 x 128
+// tiles than the chip holds at a time (512) and it leaves not much more of its outputs unused.  us with it and without:
+// 16384 x 4096 x 4096 158 / 183, 4096^3 43 / 50, 3584 x 4096 x 4096 42 / 48; 2048 x 4096 x 4096 (512) 37 / 30.
+static bool mx4_large(long long rows, int N) {
+  const long long small = ((rows + 127) / 128) * ((N + 127LL) / 128), big = ((rows + 255) / 256) * ((N + 255LL) / 256);
+  return small > 512 && 32 * big <= 9 * small;
+}
+static size_t mx4_quant_bytes(int x_dtype, long long rows, int K, int N) {
+  return x_dtype == CSMRI_MX4 || mx4_packs(rows, N) ? 0 : (size_t)rows * (mx4_code_bytes(K) + mx4_scale_bytes(K));
 }
 extern "C" size_t csmri_mx4_linear_work_bytes(int x_dtype, long long rows, int K, int N) {
   if (rows <= 0 || K <= 0 || N <= 0) return 0;
   const int s = mx4_splits(rows, K, N);
-  return mx4_quant_bytes(x_dtype, rows, K) + (s > 1 ? (size_t)s * rows * ((N + 7) / 8 * 8) * sizeof(float) : 0);
+  return mx4_quant_bytes(x_dtype, rows, K, N) + (s > 1 ? (size_t)s * rows * ((N + 7) / 8 * 8) * sizeof(float) : 0);
 }
 
 extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, const uint8_t* x_scales, long long rows, int K,
                                 const void* w_codes, const uint8_t* w_scales, int N, const float* bias, float slope,
                                 void* out, int out_dtype, int out_pix_stride, void* work, void* stream) {
-  CSMRI_CHECK_ARG(rows >= 0 && K > 0 && K % 8 == 0 && N > 0 && N <= 0x7ffffff0 && (out_dtype == CSMRI_F32 || out_dtype == CSMRI_BF16));
+  CSMRI_CHECK_ARG(rows >= 0 && K > 0 && K % 8 == 0 && K <= MX4_MAX_K && N > 0 && N <= 0x7ffffff0 && (out_dtype == CSMRI_F32 || out_dtype == CSMRI_BF16));
   const int npad = (N + 7) / 8 * 8;
   CSMRI_CHECK_ARG(out_pix_stride >= npad && w_codes && w_scales);
   CSMRI_CHECK_ARG(x_dtype == CSMRI_MX4 ? true : mx4_shape_ok(rows, K, x_pix_stride, x_dtype));
@@ -533,12 +552,12 @@ extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, co
   hipStream_t st = (hipStream_t)stream;
   if (x_dtype == CSMRI_MX4) {
     p.xq = (const char*)x; p.xs = x_scales;
-  } else if (rows > MX4_QUANT_ROWS) {
+  } else if (!mx4_packs(rows, N)) {
     p.xq = (const char*)work; p.xs = (const unsigned char*)work + (size_t)rows * p.cb;
     const int rc = csmri_mx4_quantize(x_dtype, x, x_pix_stride, rows, K, (void*)p.xq, (uint8_t*)p.xs, stream);
     if (rc != CSMRI_OK) return rc;
   }
-  if (rows <= MX4_SKINNY_ROWS) {
+  if (mx4_few(rows, N)) {
     const dim3 g((npad + 15) / 16), b(512);
     if (!p.xq) {
       if (x_dtype == CSMRI_F32) hipLaunchKernelGGL((mx4_skinny_kernel<1, CSMRI_F32>), g, b, 0, st, p);
@@ -551,10 +570,8 @@ extern "C" int csmri_mx4_linear(int x_dtype, const void* x, int x_pix_stride, co
   }
   p.splits = mx4_splits(rows, K, N);
   p.schunk = p.splits > 1 ? 4 * (((K + 511) / 512 + p.splits - 1) / p.splits) : p.ksteps;
-  p.slab = (float*)((char*)work + mx4_quant_bytes(x_dtype, rows, K));
-  // the large tile reads each operand half as often and needs a CU to itself: taken once there is one for each CU
-  const long long big = ((rows + 255) / 256) * ((N + 255) / 256);
-  const int rc = big >= 256 ? mx4_gemm_launch<4, 2, 2, 4, 2, false>(p, st) : mx4_gemm_launch<2, 2, 2, 2, 2, false>(p, st);
+  p.slab = (float*)((char*)work + mx4_quant_bytes(x_dtype, rows, K, N));
+  const int rc = mx4_large(rows, N) ? mx4_gemm_launch<4, 2, 2, 4, 2>(p, st) : mx4_gemm_launch<2, 2, 2, 2, 2>(p, st);
   if (rc != CSMRI_OK || p.splits == 1) return rc;
   const long long blocks = (rows * (npad / 4) + 255) / 256;
   hipLaunchKernelGGL(mx4_join_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p);

@@ -391,6 +391,28 @@ def test_4bit_product(ops, m, k, n, dtype):
     close(y[:, :n], ref, tol + 1e-300, 'y')
 
 
+# beside the limits between the ways of multiplying: few rows with many outputs, splits of the channels, both tiles, bands
+# of tiles that end early
+LIMIT_SIZES = [(3, 264, 8200), (16, 136, 16400), (64, 1024, 4096), (64, 1024, 4104), (64, 4608, 264), (100, 4232, 512), (1100, 2056, 136),
+               (2200, 264, 4100), (2176, 136, 4096), (66000, 72, 100)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('kept', [False, True], ids=['x', 'quantised'])
+@pytest.mark.parametrize('m,k,n', LIMIT_SIZES)
+def test_4bit_product_beside_the_limits(ops, m, k, n, kept):
+  x = pixels(m, k, torch.bfloat16, m + k)
+  w = torch.randn(n, k, generator=torch.Generator().manual_seed(n)) / k ** 0.5
+  bias = torch.randn(n, generator=torch.Generator().manual_seed(n + 1))
+  xq, wq = B.mx4(x), B.mx4(w)
+  y = ops.mx4_linear(ops.mx4_quantize(x.cuda()) if kept else x.cuda(), ops.mx4_quantize(w.cuda()), bias.cuda(), 0.25, torch.float32)
+  v = xq @ wq.t() + bias.double()
+  ref = torch.where(v > 0, v, 0.25 * v)
+  tol = (2 * ((k + 127) // 128 + 8) + 8) * U * (xq.abs() @ wq.abs().t()) + 2 * U * v.abs() + U * ref.abs()
+  close(y[:, :n], ref, tol + 1e-300, 'y')
+  assert not y[:, n:].any()
+
+
 @pytest.mark.gpu
 def test_4bit_product_of_every_code_pair_is_exact(ops):
   """Small multiples of 1/2 with unit scales: every product and sum is a short binary fraction, so the result is exact;
