@@ -513,12 +513,13 @@ static int mx4_splits(long long rows, int K, int N) {
   }
   return best;
 }
-// The 256 x 256 tile reads each operand half as often and has a CU to itself.  It is taken where there are more 128 x 128
-// tiles than the chip holds at a time (512) and it leaves not much more of its outputs unused.  us with it and without:
-// 16384 x 4096 x 4096 158 / 183, 4096^3 43 / 50, 3584 x 4096 x 4096 42 / 48; 2048 x 4096 x 4096 (512) 37 / 30.
+// The 256 x 256 tile reads each operand half as often and has a CU to itself; two of the 128 x 128 ones share one.  At 4096
+// channels a round of 256 large tiles takes 40 us, 512 small ones 24 us and 6 us for the first and last, and those need
+// not come in whole rounds.  us with large tiles and with small ones: 16384 x 4096 x 4096 157 / 183, 4096^3 43 / 50,
+// 3584 x 4096 x 4096 40 / 49; 2048 x 4096 x 4096 37 / 30, 16384 x 2048 x 1100 41 / 35, 131072 x 512 x 128 26 / 18.
 static bool mx4_large(long long rows, int N) {
   const long long small = ((rows + 127) / 128) * ((N + 127LL) / 128), big = ((rows + 255) / 256) * ((N + 255LL) / 256);
-  return small > 512 && 32 * big <= 9 * small;
+  return 40 * 512 * ((big + 255) / 256) < 6 * 512 + 24 * small;
 }
 static size_t mx4_quant_bytes(int x_dtype, long long rows, int K, int N) {
   return x_dtype == CSMRI_MX4 || mx4_packs(rows, N) ? 0 : (size_t)rows * (mx4_code_bytes(K) + mx4_scale_bytes(K));
