@@ -467,8 +467,8 @@ extern "C" int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride,
   p.splits = splits; p.slab = slab; p.dw = dw; p.db = db; p.accumulate = accumulate;
   p.chunk = ((npix + splits - 1) / splits + 63) / 64 * 64;
   const long long grid = (long long)p.ntiles * p.ctiles * splits;
-  // offsets inside a step are 32 bits
-  if (grid > 0x7fffffff || (long long)dy_pix_stride * 4 * 32 > 0x7fffffff || (long long)Cin * 32 > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
+  // offsets inside a step, of 64 pixels (32 of an fp32 dY), are 32 bits
+  if (grid > 0x7fffffff || (long long)dy_pix_stride * 4 * 32 > 0x7fffffff || (long long)Cin * 64 > 0x7fffffff) return CSMRI_E_UNSUPPORTED;
   const int rc = dy_dtype == CSMRI_F32 ? a8w_dispatch<CSMRI_F32>(t, p, (unsigned)grid, st)
                                        : a8w_dispatch<CSMRI_BF16>(t, p, (unsigned)grid, st);
   if (rc != CSMRI_OK || splits == 1) return rc;

@@ -151,6 +151,14 @@ def test_entry_points_refuse_bad_arguments():
   assert raw('csmri_mx4_linear_work_bytes')(1, 200, 136, 24) == 200 * (128 + 16) and raw('csmri_mx4_linear_work_bytes')(4, 200, 136, 24) == 0
 
 
+def test_weight_gradient_refuses_rows_beyond_32_bit_offsets():
+  import csmri_hip
+  wg = csmri_hip.lib.raw('csmri_act8_wgrad')
+  p, wide = 1 << 20, 40000000                     # 64 rows of that many codes are more than 2^31 bytes
+  assert wg(1, p, 16, p, p, 64, 16, wide, 16, wide, 1, None, p, None, 0, None) == -2
+  assert wg(0, p, 1 << 25, p, p, 64, 16, 16, 16, 16, 1, None, p, None, 0, None) == -2
+
+
 def test_operators_refuse_host_tensors_and_shapes():
   import csmri_hip
   ops = csmri_hip.ops
