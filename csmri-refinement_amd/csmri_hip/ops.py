@@ -609,6 +609,8 @@ def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
   [C_real]; channels behind C_real are padding (zero in z).  ``keep8``: ``saved`` holds x in 8 bits, written by the same
   pass, instead of x."""
   xr, n, c, ps = _pixels(x)
+  if keep8 and slope < 0:
+    raise ValueError('csmri_hip: layer_norm with keep8 needs a slope of 0 or more (the backward pass reads the sign of z)')
   c_real = gamma.shape[0]
   gamma, beta = _vector(gamma, c_real, 'gamma'), _vector(beta, c_real, 'beta')
   dev = x.device

@@ -417,6 +417,7 @@ extern "C" int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const 
   }
   CSMRI_CHECK_ARG(dz && (x != NULL) != (q8 != NULL) && (!q8 || (s8 && stats)) && (!x || x_pix_stride >= C));
   CSMRI_CHECK_ARG(slope == 1.f || x || z);                  // the sign of y is not to be had from rounded inputs
+  CSMRI_CHECK_ARG(slope >= 0.f || !z);                      // nor from z where negative outputs turn positive
   CSMRI_CHECK_ARG(!dgamma || partial);
   CSMRI_CHECK_ARG(!dx || (dx != dz && dx != x && dx != z));
   if (!ln_aligned(dz, dz_pix_stride, dtype) || (x && !ln_aligned(x, x_pix_stride, dtype)) ||

@@ -656,7 +656,8 @@ int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z, int z_pix_
                  float* stats, void* q8, uint8_t* s8, void* stream);
 /* Backward: dy = dz * (y > 0 ? 1 : slope), t = dy gamma, dx = r (t - mean_c t - h mean_c (t h)),
  * dgamma = sum_p dy h, dbeta = sum_p dy.  The input is either x (m and r are computed again) or q8 / s8 with the
- * forward's stats; with the kept form and slope != 1, z is needed for the sign of y (optional otherwise).  dx may be
+ * forward's stats; with the kept form and slope != 1, z is needed for the sign of y, which it has where slope >= 0
+ * (E_ARG below); optional otherwise.  dx may be
  * NULL; dgamma and dbeta (both or neither, [C_real], added to where accumulate != 0) need partial:
  * [csmri_ln_bwd_rows(npix, C)][2][C_real] fp32.  Fixed summation order. */
 int csmri_ln_bwd_rows(long long npix, int C);

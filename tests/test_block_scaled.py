@@ -159,6 +159,14 @@ def test_weight_gradient_refuses_rows_beyond_32_bit_offsets():
   assert wg(0, p, 1 << 25, p, p, 64, 16, 16, 16, 16, 1, None, p, None, 0, None) == -2
 
 
+def test_layer_norm_backward_refuses_the_sign_of_z_under_a_negative_slope():
+  import csmri_hip
+  bw = csmri_hip.lib.raw('csmri_ln_bwd')
+  p = 1 << 20
+  kept = [0, p, 16, None, 0, p, p, p, 2 * p, 16, 3 * p, 16, 4, 16, 13, p, 1e-5, -0.5, p, p, p, 0, None]
+  assert bw(*kept) == -1
+
+
 def test_operators_refuse_host_tensors_and_shapes():
   import csmri_hip
   ops = csmri_hip.ops
@@ -650,3 +658,28 @@ def test_two_streams_at_once(ops):
     torch.cuda.synchronize()
     for a, b in zip(want, got):
       assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_layer_norm_with_a_negative_slope(ops):
+  """From x itself any slope has its gradient; from the kept form a negative one is refused."""
+  x, gz = pixels(37, 24, torch.float32, 61), pixels(37, 24, torch.float32, 62)
+  gamma, beta = torch.linspace(0.5, 1.5, 24), torch.linspace(-0.3, 0.3, 24)
+  with pytest.raises(ValueError):
+    ops.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), slope=-0.5, keep8=True)
+  z, saved = ops.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), slope=-0.5)
+  got = ops.layer_norm_bwd(gz.cuda(), saved)
+  ref, h, mean, r = B.layer_norm(x, gamma, beta, 1e-5, -0.5)
+  y = h * gamma.double() + beta.double()
+  dh = ln_bounds(x, gamma, 1e-5)
+  dy = gamma * dh + 4 * U * (h * gamma).abs() + 4 * U * beta.abs()
+  assert (y.abs() > dy).all()                     # no output is so near to zero that rounding could turn its sign
+  close(z, ref, U * ref.abs() + dy, 'z')
+  gate = torch.where(y > 0, 1.0, -0.5).double()
+  rgx, rdg, rdb = B.layer_norm_bwd(gz, h, r, gate, gamma)
+  gg = (gz.double() * gate).abs()
+  t, m1 = gg * gamma.double(), lambda v: v.mean(1, keepdim=True)
+  tol = r * (64 * U * (t + m1(t) + 2 * h.abs() * m1(t * h.abs())) + dh * m1(t * h.abs()) + h.abs() * m1(t * dh)) + 64 * U * rgx.abs()
+  close(got[0], rgx, U * rgx.abs() + tol, 'gx')
+  close(got[1], rdg, 64 * U * (gg * h.abs()).sum(0) + (gg * dh).sum(0), 'dgamma')
+  close(got[2], rdb, 64 * U * gg.sum(0), 'dbeta')
