@@ -449,7 +449,7 @@ def _pixels(t):
         ps, span = st, st * size
       else:
         ok, span = ok and st == span, span * size
-    ok = ok and ps >= c and ps * t.element_size() % 16 == 0
+    ok = ok and c <= ps < 2 ** 31 and ps * t.element_size() % 16 == 0
   if not ok or t.data_ptr() % 16:
     t, ps = t.contiguous(), c
     if t.data_ptr() % 16:
@@ -477,12 +477,33 @@ def _vector(t, n, what):
   return t if t.is_contiguous() else t.contiguous()
 
 
+def _prod(shape):
+  n = 1
+  for k in shape:
+    n *= k
+  return n
+
+
+def _into(t, n, what):
+  """``t``, a buffer that a kernel writes ``n`` fp32 values to."""
+  if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+    raise ValueError('csmri_hip: %s has to be contiguous fp32 of %d elements, got %s %s' % (what, n, t.dtype, tuple(t.shape)))
+  return t
+
+
 class Act8(object):
   """An activation tensor kept in 8 bits (csmri_act8_save): ``q`` uint8 [pixels, C], ``s`` uint8 [pixels, ceil(C / 32)],
   ``shape`` and ``dtype`` of what was saved."""
 
   def __init__(self, q, s, shape, dtype):
+    n, c = q.shape
+    if q.dtype != torch.uint8 or s.dtype != torch.uint8 or tuple(s.shape) != (n, (c + 31) // 32) or \
+        not (q.is_contiguous() and s.is_contiguous()):
+      raise ValueError('csmri_hip: kept codes and scales have to be contiguous uint8 [pixels, C] and [pixels, ceil(C / 32)], '
+                       'got %s %s and %s %s' % (q.dtype, tuple(q.shape), s.dtype, tuple(s.shape)))
     self.q, self.s, self.shape, self.dtype = q, s, tuple(shape), dtype
+    if not self.shape or self.shape[-1] != c or _prod(self.shape) != n * c:
+      raise ValueError('csmri_hip: kept codes of %s for a tensor of %s' % (tuple(q.shape), self.shape))
 
 
 def _act8_buffers(n, c, device):
@@ -517,7 +538,13 @@ def act8_wgrad(a, gy, cout=None, cin=None, want_bias=True, dw=None, db=None, acc
   cin_p = a.shape[-1]
   cout, cin = cp if cout is None else cout, cin_p if cin is None else cin
   dev = gy.device
-  if dw is None:
+  if dw is not None:
+    _into(dw, cout * cin, 'dw')
+    if db is not None:
+      _into(db, cout, 'db')
+  elif db is not None:
+    raise ValueError('csmri_hip: act8_wgrad writes db only next to a dw')
+  else:
     dw, accumulate = torch.empty(cout, cin, dtype=torch.float32, device=dev), False
     db = torch.empty(cout, dtype=torch.float32, device=dev) if want_bias else None
   splits = lib.raw('csmri_act8_wgrad_splits')(dt_of(gr), n, cp, cin_p)
@@ -541,10 +568,14 @@ class Mx4(object):
                          (what, k, nb, t.dtype, tuple(t.shape)))
       if not t.is_contiguous() or t.data_ptr() % 16:
         raise ValueError('csmri_hip: 4-bit %s have to be contiguous and 16-byte aligned' % what)
-    if k % 8:
+    if k <= 0 or k % 8:
       raise ValueError('csmri_hip: 4-bit rows hold a multiple of 8 channels, got %d' % k)
+    if codes.get_device() != scales.get_device():
+      raise RuntimeError('csmri_hip: operands on %s and %s' % (codes.device, scales.device))
     self.codes, self.scales, self.k = codes, scales, k
     self.shape = (codes.shape[0], k) if shape is None else tuple(shape)
+    if not self.shape or self.shape[-1] != k or _prod(self.shape) != codes.shape[0] * k:
+      raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (codes.shape[0], self.shape))
 
 
 def mx4_quantize(x, out=None):
@@ -644,11 +675,16 @@ def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None
   gx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if want_x else None
   partial = None
   if want_affine:
-    if dgamma is None:
+    if (dgamma is None) != (dbeta is None):
+      raise ValueError('csmri_hip: layer_norm_bwd writes dgamma and dbeta, both or neither')
+    if dgamma is not None:
+      _into(dgamma, saved.c_real, 'dgamma')
+      _into(dbeta, saved.c_real, 'dbeta')
+    else:
       dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
                                    torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
     partial = torch.empty(lib.raw('csmri_ln_bwd_rows')(n, c), 2, saved.c_real, dtype=torch.float32, device=dev)
-  _launch(gz, (saved.snap, xr, zr, dgamma, dbeta), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps,
+  _launch(gz, (saved.snap, xr, zr, kept.q if kept else None, dgamma, dbeta), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps,
           ptr(kept.q) if kept else 0, ptr(kept.s) if kept else 0, ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c,
           saved.c_real, saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
           ptr(dbeta) if want_affine else 0, int(bool(accumulate)))

@@ -182,6 +182,23 @@ def test_operators_refuse_host_tensors_and_shapes():
       ops.Mx4(*args)
 
 
+def test_kept_forms_refuse_what_does_not_fit_their_shape():
+  import csmri_hip
+  ops = csmri_hip.ops
+  z = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+  ops.Act8(z(6, 40), z(6, 2), (2, 3, 40), torch.bfloat16)
+  for q, s, shape in ((z(6, 40), z(6, 1), (6, 40)), (z(6, 40), z(5, 2), (6, 40)), (z(6, 40).int(), z(6, 2), (6, 40)),
+                      (z(40, 6).t(), z(6, 2), (6, 40)), (z(6, 40), z(6, 2), (7, 40)), (z(6, 40), z(6, 2), (12, 20)), (z(6, 40), z(6, 2), ())):
+    with pytest.raises(ValueError):
+      ops.Act8(q, s, shape, torch.bfloat16)
+  for shape in ((7, 136), (6, 64), (2, 136), ()):
+    with pytest.raises(ValueError):
+      ops.Mx4(z(6, 128), z(6, 16), 136, shape)
+  for k in (0, -8):
+    with pytest.raises(ValueError):
+      ops.Mx4(z(6, 0), z(6, 0), k)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # GPU
 # ---------------------------------------------------------------------------------------------------------------------
@@ -683,3 +700,21 @@ def test_layer_norm_with_a_negative_slope(ops):
   close(got[0], rgx, U * rgx.abs() + tol, 'gx')
   close(got[1], rdg, 64 * U * (gg * h.abs()).sum(0) + (gg * dh).sum(0), 'dgamma')
   close(got[2], rdb, 64 * U * gg.sum(0), 'dbeta')
+
+
+@pytest.mark.gpu
+def test_gradient_buffers_that_do_not_fit_are_refused(ops):
+  x = torch.randn(12, 24, device='cuda')
+  f = lambda *s, **k: torch.zeros(*s, device='cuda', **k)
+  kept = ops.act8_save(x)
+  for kw in (dict(dw=f(24, 23)), dict(dw=f(24, 24).bfloat16()), dict(dw=f(24, 48)[:, ::2]), dict(dw=f(24, 24), db=f(23)),
+             dict(dw=f(24, 24), db=f(24).double()), dict(db=f(24))):
+    with pytest.raises(ValueError):
+      ops.act8_wgrad(kept, x, **kw)
+  z, saved = ops.layer_norm(x, f(24), f(24))
+  for kw in (dict(dgamma=f(24)), dict(dbeta=f(24)), dict(dgamma=f(23), dbeta=f(24)), dict(dgamma=f(24), dbeta=f(48)[::2]),
+             dict(dgamma=f(24).half(), dbeta=f(24))):
+    with pytest.raises(ValueError):
+      ops.layer_norm_bwd(x, saved, **kw)
+  a, b = ops.act8_wgrad(kept, x, dw=f(24, 24, 1, 1), db=f(24)), ops.act8_wgrad(kept, x)
+  assert torch.equal(a[0].view(24, 24), b[0]) and torch.equal(a[1], b[1])
