@@ -1661,10 +1661,13 @@ class ConvBnAct(torch.autograd.Function):
 
 class LayerNormAct(torch.autograd.Function):
   """layer_norm as an autograd node: z = lrelu(layer norm of x over its channels).  ``keep8``: x is kept in 8 bits.
-  Like the BatchNorm node's, the affine gradients are accumulated into gamma.grad / beta.grad by the kernels."""
+  Like the BatchNorm node's, the affine gradients are accumulated into gamma.grad / beta.grad by the kernels, so the two
+  have to be leaves (Parameters)."""
 
   @staticmethod
   def forward(ctx, x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
+    if not (gamma.is_leaf and beta.is_leaf):
+      raise ValueError('csmri_hip: LayerNormAct writes the gradients of gamma and beta itself: they have to be leaf tensors')
     z, sv = layer_norm(x, gamma, beta, eps, slope, keep8)
     ctx.gamma, ctx.beta = gamma, beta
     ctx.affine_req = (gamma.requires_grad, beta.requires_grad)

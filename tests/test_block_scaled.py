@@ -718,3 +718,16 @@ def test_gradient_buffers_that_do_not_fit_are_refused(ops):
       ops.layer_norm_bwd(x, saved, **kw)
   a, b = ops.act8_wgrad(kept, x, dw=f(24, 24, 1, 1), db=f(24)), ops.act8_wgrad(kept, x)
   assert torch.equal(a[0].view(24, 24), b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+def test_layer_norm_node_refuses_computed_parameters(ops):
+  """Its gradients go to gamma.grad: through a computed gamma they would not reach what it was computed from."""
+  x = torch.randn(4, 16, device='cuda', requires_grad=True)
+  w, b = torch.ones(16, device='cuda', requires_grad=True), torch.zeros(16, device='cuda', requires_grad=True)
+  with pytest.raises(ValueError):
+    ops.LayerNormAct.apply(x, w * 2, b)
+  with pytest.raises(ValueError):
+    ops.LayerNormAct.apply(x, w, b + 1)
+  ops.LayerNormAct.apply(x, w, b.detach()).sum().backward()
+  assert w.grad is not None and b.grad is None
