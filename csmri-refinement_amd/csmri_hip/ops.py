@@ -291,6 +291,10 @@ class PackGroup(object):
         self.repack(mode)
     if any(l._bias_pad is not None and l._bias_pad[0] != _weight_epoch(l) for l in self.layers):
       self.refresh_biases()
+    if modes is None:
+      for l in self.layers:
+        if l._pack4 is not None:
+          l._pack_mx4()
 
   def refresh_biases(self):
     """One multi-tensor copy of every stale member bias into its zero-padded fp32 buffer (the fallback: a re-pack

@@ -731,3 +731,39 @@ def test_layer_norm_node_refuses_computed_parameters(ops):
     ops.LayerNormAct.apply(x, w, b + 1)
   ops.LayerNormAct.apply(x, w, b.detach()).sum().backward()
   assert w.grad is not None and b.grad is None
+
+
+@pytest.mark.gpu
+def test_captured_forward_follows_loaded_weights(ops):
+  """refresh_packs brings the 4-bit copies of replaced weights up to date in place: a captured graph reads them."""
+  from models import unet, utils
+
+  def build(seed):
+    torch.manual_seed(seed)
+    net = unet.UNET(1, 1, 2, [32, 64], [32], 'none', kernel_size=3, upsampling_mode='nn-resize-conv', padding='reflection',
+                    decoder_act_upsampling_only=True, compute_dtype='bf16').cuda().eval()
+    assert utils.set_mx4_forward(net) == 1
+    return net
+
+  net, other = build(5), build(6)
+  x = torch.randn(2, 1, 64, 64, generator=torch.Generator().manual_seed(8)).cuda()
+  with torch.no_grad():
+    first, want = net(x), other(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+      net(x)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      y = net(x)
+    graph.replay()
+    assert torch.equal(y, first) and not torch.equal(first, want)
+    net.load_state_dict(other.state_dict())
+    ops.bump_weight_epoch()
+    utils.refresh_packs(net)
+    for _ in range(2):
+      graph.replay()
+      assert torch.equal(y, want)
+      torch.cuda.synchronize()
