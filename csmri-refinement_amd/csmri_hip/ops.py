@@ -8,6 +8,7 @@ padded to a multiple of 8, pad channels zero) in the compute dtype
 (``stride(3)==1``, dense in B,H,W).
 """
 import ctypes as C
+import math
 import os
 
 import torch
@@ -468,7 +469,7 @@ def _launch(t, operands, name, *args):
     if o is not None and o.get_device() != dev:
       raise RuntimeError('csmri_hip: operands on %s and %s' % (t.device, o.device))
   st = torch._C._cuda_getCurrentRawStream(dev)
-  if dev == torch.cuda.current_device():
+  if dev == torch._C._cuda_getDevice():
     lib.call(name, *args, st)
   else:
     with torch.cuda.device(dev):
@@ -479,13 +480,6 @@ def _vector(t, n, what):
   if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n:
     raise ValueError('csmri_hip: %s has to be fp32 [%d], got %s %s' % (what, n, t.dtype, tuple(t.shape)))
   return t if t.is_contiguous() else t.contiguous()
-
-
-def _prod(shape):
-  n = 1
-  for k in shape:
-    n *= k
-  return n
 
 
 def _into(t, n, what):
@@ -506,21 +500,27 @@ class Act8(object):
       raise ValueError('csmri_hip: kept codes and scales have to be contiguous uint8 [pixels, C] and [pixels, ceil(C / 32)], '
                        'got %s %s and %s %s' % (q.dtype, tuple(q.shape), s.dtype, tuple(s.shape)))
     self.q, self.s, self.shape, self.dtype = q, s, tuple(shape), dtype
-    if not self.shape or self.shape[-1] != c or _prod(self.shape) != n * c:
+    if not self.shape or self.shape[-1] != c or math.prod(self.shape) != n * c:
       raise ValueError('csmri_hip: kept codes of %s for a tensor of %s' % (tuple(q.shape), self.shape))
 
-
-def _act8_buffers(n, c, device):
-  return (torch.empty(n, c, dtype=torch.uint8, device=device),
-          torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=device))
+  @classmethod
+  def _new(cls, x):
+    """Buffers for ``x`` (the checks of buffers from elsewhere take a tenth of a small call's time)."""
+    a = cls.__new__(cls)
+    a.shape, a.dtype, dev = x.shape, x.dtype, x.device
+    c = a.shape[-1]
+    n = x.numel() // c
+    a.q = torch.empty(n, c, dtype=torch.uint8, device=dev)
+    a.s = torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=dev)
+    return a
 
 
 def act8_save(x):
   """Keep ``x`` (bf16 / fp32) in 8 bits: e4m3 codes, one power-of-two scale per 32 channels of a pixel."""
   xr, n, c, ps = _pixels(x)
-  q, s = _act8_buffers(n, c, x.device)
-  _launch(x, (), 'csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, q.data_ptr(), s.data_ptr())
-  return Act8(q, s, x.shape, x.dtype)
+  a = Act8._new(x)
+  _launch(x, (), 'csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, a.q.data_ptr(), a.s.data_ptr())
+  return a
 
 
 def act8_restore(a, dtype=None):
@@ -578,16 +578,26 @@ class Mx4(object):
       raise RuntimeError('csmri_hip: operands on %s and %s' % (codes.device, scales.device))
     self.codes, self.scales, self.k = codes, scales, k
     self.shape = (codes.shape[0], k) if shape is None else tuple(shape)
-    if not self.shape or self.shape[-1] != k or _prod(self.shape) != codes.shape[0] * k:
+    if not self.shape or self.shape[-1] != k or math.prod(self.shape) != codes.shape[0] * k:
       raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (codes.shape[0], self.shape))
+
+  @classmethod
+  def _new(cls, x):
+    """Buffers for ``x``."""
+    m = cls.__new__(cls)
+    m.shape, dev = x.shape, x.device
+    m.k = k = m.shape[-1]
+    n = x.numel() // k
+    m.codes = torch.empty(n, 64 * ((k + 127) // 128), dtype=torch.uint8, device=dev)
+    m.scales = torch.empty(n, 16 * ((k + 511) // 512), dtype=torch.uint8, device=dev)
+    return m
 
 
 def mx4_quantize(x, out=None):
   """``x`` [..., k] (bf16 / fp32) as 4-bit rows; ``out``: an Mx4 of the same size to overwrite."""
   xr, n, c, ps = _pixels(x)
   if out is None:
-    out = Mx4(torch.empty(n, lib.raw('csmri_mx4_code_bytes')(c), dtype=torch.uint8, device=x.device),
-              torch.empty(n, lib.raw('csmri_mx4_scale_bytes')(c), dtype=torch.uint8, device=x.device), c, x.shape)
+    out = Mx4._new(x)
   elif out.k != c or out.codes.shape[0] != n:
     raise ValueError('csmri_hip: 4-bit buffers of %s for a tensor of %s' % (out.shape, tuple(x.shape)))
   _launch(x, (out.codes, out.scales), 'csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, out.codes.data_ptr(),
@@ -636,7 +646,7 @@ class LNSaved(object):
 
   def __init__(self, x, kept, stats, snap, shape, dtype, c_real, eps, slope):
     self.x, self.kept, self.stats, self.snap = x, kept, stats, snap
-    self.shape, self.dtype, self.c_real, self.eps, self.slope = tuple(shape), dtype, c_real, eps, slope
+    self.shape, self.dtype, self.c_real, self.eps, self.slope = shape, dtype, c_real, eps, slope
 
 
 def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
@@ -646,17 +656,17 @@ def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
   xr, n, c, ps = _pixels(x)
   if keep8 and slope < 0:
     raise ValueError('csmri_hip: layer_norm with keep8 needs a slope of 0 or more (the backward pass reads the sign of z)')
-  c_real = gamma.shape[0]
+  c_real, eps, slope = gamma.shape[0], float(eps), float(slope)
   gamma, beta = _vector(gamma, c_real, 'gamma'), _vector(beta, c_real, 'beta')
   dev = x.device
   z = torch.empty(x.shape, dtype=x.dtype, device=dev)
   snap = torch.empty(2, c, dtype=torch.float32, device=dev)
-  q, s = _act8_buffers(n, c, dev) if keep8 else (None, None)
+  kept = Act8._new(x) if keep8 else None
   stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
   _launch(x, (gamma, beta), 'csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
-          beta.data_ptr(), float(eps), float(slope), snap.data_ptr(), ptr(stats), ptr(q), ptr(s))
-  return z, LNSaved(None if keep8 else xr, Act8(q, s, x.shape, x.dtype) if keep8 else None, stats, snap, x.shape,
-                    x.dtype, c_real, float(eps), float(slope))
+          beta.data_ptr(), eps, slope, snap.data_ptr(), ptr(stats), kept.q.data_ptr() if keep8 else 0,
+          kept.s.data_ptr() if keep8 else 0)
+  return z, LNSaved(None if keep8 else xr, kept, stats, snap, x.shape, x.dtype, c_real, eps, slope)
 
 
 def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None, dbeta=None, accumulate=False):
