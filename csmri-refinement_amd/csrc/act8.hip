@@ -1,7 +1,8 @@
 // Activations kept for the backward pass in 8 bits (micro.h: e4m3 elements, one power-of-two scale per 32 channels of a
 // pixel: 1.03 bytes a channel instead of 2 or 4), and the weight gradient of a 1 x 1 convolution that reads them.
 //
-// Save and restore are streams: one read, one write, bound by HBM.
+// Save and restore are streams: one read, one write, bound by HBM (16384 x 2048 bf16: 17 us for 102 MB; 131072 x 64: 6.7 and
+// 5.9 us for 25 MB, a third of it the launch).  A thread keeps its channels and has four rows under way.
 #include "micro.h"
 #include "wgrad_params.h"
 #include <type_traits>
@@ -204,8 +205,9 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
 // time.  Both operands pass through registers into one of two LDS stages, the input's codes becoming bf16 on the way, and
 // are loaded a step ahead of that.  (LDS-DMA would spare dY the registers, but the compiler lets no transposed read pass a
 // pending one; a second set of registers, to load two steps ahead, costs more in occupancy than it hides.)  Bound by the
-// matrix unit and the steps around it: of the 192 us at 2048 x 2048 channels and 16384 pixels, a loop of the products,
-// barriers and stores alone takes 132.
+// matrix unit and the staging beside it: 165 - 177 us at 2048 x 2048 channels and 16384 pixels (800 TFLOP/s), where a loop
+// of products and barriers alone takes 120 - 132.  LDS is not what bounds it: images turned over in
+// registers, [channel][pixel], and read 16 bytes at a time halve its reads and took 178.
 //
 // GK = 2: a second set of waves takes every other step, with stages of its own, and hands its sums over at the end -- the
 // occupancy of two workgroups with the partial sums of one, which otherwise cost as much as the small layers' operands.
@@ -413,7 +415,8 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
 
 // Tile: 64 or 128 a side by the channel counts; 256 x 256 (an fp32 dY's three planes do not fit it),
 // which reads LDS a third less per product, where 2048 pixels a split still leave three quarters of the CUs a workgroup.
-// 2048 x 2048 channels, 16384 pixels: 192 us against 225 with 128 x 128; 512 x 512, 8192 pixels: 46 against 35.
+// 2048 x 2048 channels, 16384 pixels, with the partial sums: 189 us against 225 with 128 x 128; 512 x 512, 8192 pixels:
+// 46 against 30.
 struct A8WTile { int bn, bc; };
 static A8WTile a8w_tile(int dy_dtype, long long npix, int Cout, int Cin) {
   if (dy_dtype == CSMRI_BF16 && Cout > 128 && Cin > 128 &&

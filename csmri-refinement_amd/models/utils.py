@@ -66,7 +66,8 @@ def set_mx4_forward(module, on=True):
 
 def set_keep8(module, on=True):
   """Keep the inputs of every trainable convolution under ``module`` in 8 bits for their weight gradients
-  (ops.ConvLayer.keep8); returns how many layers that concerns.  Outputs and data gradients do not change."""
+  (ops.ConvLayer.keep8); returns how many layers that concerns.  Outputs and data gradients do not change.  Conv blocks
+  that run as one launch and replayed sub-batches keep theirs as they are: those inputs are held for other reasons."""
   return _set_layer_flag(module, 'keep8', on, lambda layer: True)
 
 

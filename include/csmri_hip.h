@@ -681,7 +681,8 @@ int csmri_act8_restore(const void* q8, const uint8_t* s8, long long npix, int C,
  * dw: fp32 [Cout_real][Cin_real]; db: fp32 [Cout_real] or NULL; Cout, Cin: padded channel counts of dy and of the kept
  * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts.
  * splits: csmri_act8_wgrad_splits; slab: csmri_act8_wgrad_slab_bytes (NULL when that is 0).  Fixed summation order.
- * npix == 0 leaves zeros (or what was there, with accumulate). */
+ * npix == 0 leaves zeros (or what was there, with accumulate).  64 pixels of dy and of q8 stay below 2^31 bytes
+ * (E_UNSUPPORTED otherwise). */
 int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin);
 size_t csmri_act8_wgrad_slab_bytes(int splits, int Cout_real, int Cin_real);
 int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride, const void* q8, const uint8_t* s8, long long npix,
@@ -694,7 +695,7 @@ int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride, const void
  * csmri_mx4_scale_bytes(K) = 16 ceil(K / 512) scale bytes; padding is code 0 and any scale but 255 (the quantiser writes
  * 2^0).  codes, scales: 16-byte aligned, dense rows.
  *   e = max(floor(log2(max |x| of the block)), -100), scale 2^(e - 2), code = e2m1_rne(x / scale), saturating at 6
- * A block with a NaN or an infinity: scale 255, all of it reads NaN.  K % 8 == 0.
+ * A block with a NaN or an infinity: scale 255, all of it reads NaN.  K % 8 == 0, K <= 2^24.
  * ---------------------------------------------------------------------- */
 int csmri_mx4_code_bytes(int K);
 int csmri_mx4_scale_bytes(int K);

@@ -270,7 +270,7 @@ def ln_bounds(x, gamma, eps):
   return dh
 
 
-LN_SIZES = [(1, 1), (64, 8), (5, 13), (70, 100), (33, 32), (9, 512), (6, 520), (17, 1024), (5, 2000), (3, 2056), (2, 8192), (3000, 24), (4, 4100)]
+LN_SIZES = [(1, 1), (64, 8), (97, 64), (129, 64), (8, 1024), (4, 2048), (5, 13), (70, 100), (33, 32), (9, 512), (6, 520), (17, 1024), (5, 2000), (3, 2056), (2, 8192), (3000, 24), (4, 4100)]
 
 
 @pytest.mark.gpu
@@ -337,6 +337,22 @@ def test_layer_norm_strides_accumulation_and_parts(ops):
               lambda: ops.layer_norm_bwd(gz, ops.layer_norm(dense, gamma, beta, slope=0.2, keep8=True)[1])):
     with pytest.raises((ValueError, RuntimeError)):
       bad()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('n', [1, 64, 128, 129])
+def test_layer_norm_few_rows_accumulate(ops, n):
+  """One workgroup writes the affine gradients itself, several through partial rows: either adds where asked to."""
+  x, gz = pixels(n, 64, torch.float32, n).cuda(), pixels(n, 64, torch.float32, n + 1).cuda()
+  _, saved = ops.layer_norm(x, torch.ones(64, device='cuda'), torch.zeros(64, device='cuda'))
+  _, dg, db = ops.layer_norm_bwd(gz, saved)
+  a, b = torch.full((64,), 3.0, device='cuda'), torch.full((64,), -2.0, device='cuda')
+  for k in (1, 2):
+    want_a, want_b = a + dg, b + db
+    ops.layer_norm_bwd(gz, saved, dgamma=a, dbeta=b, accumulate=True)
+    assert torch.equal(a, want_a) and torch.equal(b, want_b)
+  ops.layer_norm_bwd(gz, saved, dgamma=a, dbeta=b)
+  assert torch.equal(a, dg) and torch.equal(b, db)
 
 
 @pytest.mark.gpu
