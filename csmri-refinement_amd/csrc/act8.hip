@@ -426,11 +426,20 @@ static A8WTile a8w_tile(int dy_dtype, long long npix, int Cout, int Cin) {
 extern "C" int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin) {
   if (npix <= 0 || Cout <= 0 || Cin <= 0) return 1;
   const A8WTile t = a8w_tile(dy_dtype, npix, Cout, Cin);
-  const long long tiles = (long long)cdiv(Cout, t.bn) * cdiv(Cin, t.bc);
-  long long s = 256 / tiles;                                  // one workgroup of eight waves a CU
-  const long long most = npix / 512;                          // at least eight steps each
-  if (s > most) s = most;
-  return s < 1 ? 1 : (int)s;
+  const long long tiles = (long long)cdiv(Cout, t.bn) * cdiv(Cin, t.bc), len = (long long)(Cout + 1) * Cin * 4;
+  const long long most = 256 / tiles < npix / 128 ? 256 / tiles : npix / 128;     // one workgroup of eight waves a CU
+  // ns: 128 pixels of a tile; partial sums, written and read, a MiB; the launch that adds them.  Measured, in us, by the
+  // number of splits: 4096 pixels, 64 to 128 channels, 1: 37, 8: 14.8, 16 - 32: 13.7; 4096, 512 to 512, 4: 26, 8: 24, 16: 26;
+  // 4096, 1024 to 1024, 2: 40, 4: 34, 8: 48; 1024, 1024 to 1024, 1: 23, 2: 25.
+  const long long step = (500 + t.bn * t.bc / 1024 * 42) * (dy_dtype == CSMRI_F32 ? 2 : 1);
+  long long best = 1, least = step * ((npix + 127) / 128);
+  for (long long c = 2; most > 1; c += c & (c - 1) ? c / 3 : c / 2) {      // 2, 3, 4, 6, 8, 12, ... and the most
+    const long long s = c < most ? c : most;
+    const long long cost = step * (((npix + s - 1) / s + 127) / 128) + 4000 + (600 * s * len >> 20);
+    if (cost < least) { least = cost; best = s; }
+    if (s == most) break;
+  }
+  return (int)best;
 }
 template <int DT, int FN, int FC, int WN, int WC, int KP, int GK> static int a8w_launch(const A8WParams& p, unsigned grid, hipStream_t st) {
   constexpr int BN = 16 * FN * WN, BC = 16 * FC * WC, LDS = GK * 2 * KP * 2 * (BN * (DT == CSMRI_F32 ? 3 : 1) + BC);
