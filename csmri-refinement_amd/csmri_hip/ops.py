@@ -233,12 +233,12 @@ class ConvLayer(object):
     """The layer's weights as 4-bit rows of ``cin_p`` channels (csmri_mx4_quantize)."""
     epoch = _weight_epoch(self)
     ent = self._pack4
-    if ent is not None and ent[0] == epoch and ent[1].codes.device == self.weight.device:
+    if ent is not None and ent[0] == epoch and ent[1].tensors()[0].device == self.weight.device:
       return ent[1]
     w = self.weight.detach().reshape(self.cout, self.cin)
     if self.cin_p != self.cin:
       w = torch.nn.functional.pad(w, (0, self.cin_p - self.cin))
-    q = mx4_quantize(w, ent[1] if ent is not None and ent[1].codes.device == self.weight.device else None)
+    q = mx4_quantize(w, ent[1] if ent is not None and ent[1].tensors()[0].device == self.weight.device else None)
     self._pack4 = (epoch, q)
     return q
 
@@ -499,36 +499,64 @@ class Act8(object):
         not (q.is_contiguous() and s.is_contiguous()):
       raise ValueError('csmri_hip: kept codes and scales have to be contiguous uint8 [pixels, C] and [pixels, ceil(C / 32)], '
                        'got %s %s and %s %s' % (q.dtype, tuple(q.shape), s.dtype, tuple(s.shape)))
-    self.q, self.s, self.shape, self.dtype = q, s, tuple(shape), dtype
+    self.buf, self._q, self._s, self.pixels, self.shape, self.dtype = None, q, s, n, tuple(shape), dtype
     if not self.shape or self.shape[-1] != c or math.prod(self.shape) != n * c:
       raise ValueError('csmri_hip: kept codes of %s for a tensor of %s' % (tuple(q.shape), self.shape))
 
   @classmethod
-  def _new(cls, x):
-    """Buffers for ``x`` (the checks of buffers from elsewhere take a tenth of a small call's time)."""
+  def _of(cls, buf, shape, dtype):
+    """Codes and scales one behind the other in ``buf``: an allocation less."""
     a = cls.__new__(cls)
-    a.shape, a.dtype, dev = x.shape, x.dtype, x.device
-    c = a.shape[-1]
-    n = x.numel() // c
-    a.q = torch.empty(n, c, dtype=torch.uint8, device=dev)
-    a.s = torch.empty(n, (c + 31) // 32, dtype=torch.uint8, device=dev)
+    a.buf, a._q, a._s, a.shape, a.dtype = buf, None, None, shape, dtype
+    a.pixels = math.prod(shape) // shape[-1]
     return a
+
+  @classmethod
+  def _new(cls, x):
+    shape = x.shape
+    c = shape[-1]
+    n = x.numel() // c
+    return cls._of(torch.empty(n * (c + (c + 31) // 32), dtype=torch.uint8, device=x.device), shape, x.dtype)
+
+  @property
+  def q(self):
+    if self._q is None:
+      c = self.shape[-1]
+      self._q = self.buf[:self.pixels * c].view(self.pixels, c)
+    return self._q
+
+  @property
+  def s(self):
+    if self._s is None:
+      c = self.shape[-1]
+      self._s = self.buf[self.pixels * c:].view(self.pixels, (c + 31) // 32)
+    return self._s
+
+  def tensors(self):
+    return (self._q, self._s) if self.buf is None else (self.buf,)
+
+  def addresses(self):
+    if self.buf is None:
+      return self._q.data_ptr(), self._s.data_ptr()
+    p = self.buf.data_ptr()
+    return p, p + self.pixels * self.shape[-1]
 
 
 def act8_save(x):
   """Keep ``x`` (bf16 / fp32) in 8 bits: e4m3 codes, one power-of-two scale per 32 channels of a pixel."""
   xr, n, c, ps = _pixels(x)
   a = Act8._new(x)
-  _launch(x, (), 'csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, a.q.data_ptr(), a.s.data_ptr())
+  _launch(x, (), 'csmri_act8_save', dt_of(xr), xr.data_ptr(), ps, n, c, *a.addresses())
   return a
 
 
 def act8_restore(a, dtype=None):
   """The values of a kept tensor in its own dtype or ``dtype``."""
   dtype = a.dtype if dtype is None else dtype
-  out = torch.empty(a.shape, dtype=dtype, device=a.q.device)
+  kept = a.tensors()
+  out = torch.empty(a.shape, dtype=dtype, device=kept[0].device)
   c = a.shape[-1]
-  _launch(out, (a.q, a.s), 'csmri_act8_restore', a.q.data_ptr(), a.s.data_ptr(), a.q.shape[0], c, dt_of(out),
+  _launch(out, kept, 'csmri_act8_restore', *a.addresses(), a.pixels, c, dt_of(out),
           out.data_ptr(), c)
   return out
 
@@ -554,7 +582,7 @@ def act8_wgrad(a, gy, cout=None, cin=None, want_bias=True, dw=None, db=None, acc
   splits = lib.raw('csmri_act8_wgrad_splits')(dt_of(gr), n, cp, cin_p)
   nbytes = lib.raw('csmri_act8_wgrad_slab_bytes')(splits, cout, cin)
   slab = torch.empty(nbytes // 4, dtype=torch.float32, device=dev) if nbytes else None
-  _launch(gy, (a.q, a.s, dw, db), 'csmri_act8_wgrad', dt_of(gr), gr.data_ptr(), ps, a.q.data_ptr(), a.s.data_ptr(), n, cp,
+  _launch(gy, a.tensors() + (dw, db), 'csmri_act8_wgrad', dt_of(gr), gr.data_ptr(), ps, *a.addresses(), n, cp,
           cin_p, cout, cin, splits, ptr(slab), dw.data_ptr(), ptr(db), int(bool(accumulate)))
   return dw, db
 
@@ -576,21 +604,42 @@ class Mx4(object):
       raise ValueError('csmri_hip: 4-bit rows hold a multiple of 8 channels, got %d' % k)
     if codes.get_device() != scales.get_device():
       raise RuntimeError('csmri_hip: operands on %s and %s' % (codes.device, scales.device))
-    self.codes, self.scales, self.k = codes, scales, k
-    self.shape = (codes.shape[0], k) if shape is None else tuple(shape)
-    if not self.shape or self.shape[-1] != k or math.prod(self.shape) != codes.shape[0] * k:
-      raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (codes.shape[0], self.shape))
+    self.buf, self._codes, self._scales, self.rows, self.k = None, codes, scales, codes.shape[0], k
+    self.shape = (self.rows, k) if shape is None else tuple(shape)
+    if not self.shape or self.shape[-1] != k or math.prod(self.shape) != self.rows * k:
+      raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (self.rows, self.shape))
 
   @classmethod
   def _new(cls, x):
-    """Buffers for ``x``."""
+    """Codes and scales of ``x`` one behind the other in ``buf``: an allocation less."""
     m = cls.__new__(cls)
-    m.shape, dev = x.shape, x.device
+    m._codes, m._scales, m.shape = None, None, x.shape
     m.k = k = m.shape[-1]
-    n = x.numel() // k
-    m.codes = torch.empty(n, 64 * ((k + 127) // 128), dtype=torch.uint8, device=dev)
-    m.scales = torch.empty(n, 16 * ((k + 511) // 512), dtype=torch.uint8, device=dev)
+    m.rows = x.numel() // k
+    m.buf = torch.empty(m.rows * (64 * ((k + 127) // 128) + 16 * ((k + 511) // 512)), dtype=torch.uint8, device=x.device)
     return m
+
+  @property
+  def codes(self):
+    if self._codes is None:
+      cb = 64 * ((self.k + 127) // 128)
+      self._codes = self.buf[:self.rows * cb].view(self.rows, cb)
+    return self._codes
+
+  @property
+  def scales(self):
+    if self._scales is None:
+      self._scales = self.buf[self.rows * 64 * ((self.k + 127) // 128):].view(self.rows, 16 * ((self.k + 511) // 512))
+    return self._scales
+
+  def tensors(self):
+    return (self._codes, self._scales) if self.buf is None else (self.buf,)
+
+  def addresses(self):
+    if self.buf is None:
+      return self._codes.data_ptr(), self._scales.data_ptr()
+    p = self.buf.data_ptr()
+    return p, p + self.rows * 64 * ((self.k + 127) // 128)
 
 
 def mx4_quantize(x, out=None):
@@ -598,17 +647,17 @@ def mx4_quantize(x, out=None):
   xr, n, c, ps = _pixels(x)
   if out is None:
     out = Mx4._new(x)
-  elif out.k != c or out.codes.shape[0] != n:
+  elif out.k != c or out.rows != n:
     raise ValueError('csmri_hip: 4-bit buffers of %s for a tensor of %s' % (out.shape, tuple(x.shape)))
-  _launch(x, (out.codes, out.scales), 'csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, out.codes.data_ptr(),
-          out.scales.data_ptr())
+  _launch(x, out.tensors(), 'csmri_mx4_quantize', dt_of(xr), xr.data_ptr(), ps, n, c, *out.addresses())
   return out
 
 
 def mx4_dequantize(m, dtype=torch.bfloat16):
   """The values 4-bit rows stand for (exact in either dtype)."""
-  out = torch.empty(m.shape, dtype=dtype, device=m.codes.device)
-  _launch(out, (m.codes, m.scales), 'csmri_mx4_dequantize', m.codes.data_ptr(), m.scales.data_ptr(), m.codes.shape[0], m.k,
+  rows = m.tensors()
+  out = torch.empty(m.shape, dtype=dtype, device=rows[0].device)
+  _launch(out, rows, 'csmri_mx4_dequantize', *m.addresses(), m.rows, m.k,
           dt_of(out), out.data_ptr(), m.k)
   return out
 
@@ -618,15 +667,14 @@ def mx4_linear(x, w, bias=None, slope=1.0, out_dtype=None):
   with 4-bit weights ``w`` (Mx4 of N rows), act the LeakyReLU of ``slope`` (1: none).  Returns [..., pad8(N)] in
   ``out_dtype`` (default: of x; bf16 for an Mx4), pad channels zero."""
   if isinstance(x, Mx4):
-    dev_t, n, k, ps, shape, xdt, xp, sp = x.codes, x.codes.shape[0], x.k, 0, x.shape, MX4, x.codes.data_ptr(), \
-        x.scales.data_ptr()
-    xr = None
+    dev_t, n, k, ps, shape, xdt, xr = x.tensors()[0], x.rows, x.k, 0, x.shape, MX4, None
+    xp, sp = x.addresses()
   else:
     xr, n, k, ps = _pixels(x)
     dev_t, shape, xdt, xp, sp = x, x.shape, dt_of(xr), xr.data_ptr(), 0
   if k != w.k:
     raise ValueError('csmri_hip: %d channels against 4-bit weights of %d' % (k, w.k))
-  cout = w.codes.shape[0]
+  cout = w.rows
   if bias is not None:
     bias = _vector(bias, cout, 'bias')
   out_dtype = out_dtype or (torch.bfloat16 if xr is None else x.dtype)
@@ -635,8 +683,7 @@ def mx4_linear(x, w, bias=None, slope=1.0, out_dtype=None):
     return y
   nbytes = lib.raw('csmri_mx4_linear_work_bytes')(xdt, n, k, cout)
   work = torch.empty(nbytes, dtype=torch.uint8, device=dev_t.device) if nbytes else None
-  _launch(dev_t, (w.codes, w.scales, bias), 'csmri_mx4_linear', xdt, xp, ps, sp, n, k, w.codes.data_ptr(),
-          w.scales.data_ptr(), cout, ptr(bias), float(slope), y.data_ptr(), dt_of(y), y.shape[-1], ptr(work))
+  _launch(dev_t, w.tensors() + (bias,), 'csmri_mx4_linear', xdt, xp, ps, sp, n, k, *w.addresses(), cout, ptr(bias), float(slope), y.data_ptr(), dt_of(y), y.shape[-1], ptr(work))
   return y
 
 
@@ -664,8 +711,7 @@ def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
   kept = Act8._new(x) if keep8 else None
   stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
   _launch(x, (gamma, beta), 'csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
-          beta.data_ptr(), eps, slope, snap.data_ptr(), ptr(stats), kept.q.data_ptr() if keep8 else 0,
-          kept.s.data_ptr() if keep8 else 0)
+          beta.data_ptr(), eps, slope, snap.data_ptr(), ptr(stats), *(kept.addresses() if keep8 else (0, 0)))
   return z, LNSaved(None if keep8 else xr, kept, stats, snap, x.shape, x.dtype, c_real, eps, slope)
 
 
@@ -697,9 +743,10 @@ def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None
     else:
       dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
                                    torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
-    partial = torch.empty(lib.raw('csmri_ln_bwd_rows')(n, c), 2, saved.c_real, dtype=torch.float32, device=dev)
-  _launch(gz, (saved.snap, xr, zr, kept.q if kept else None, dgamma, dbeta), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(), gps, ptr(xr), xps,
-          ptr(kept.q) if kept else 0, ptr(kept.s) if kept else 0, ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c,
+    rows = lib.raw('csmri_ln_bwd_rows')(n, c)        # (one: nothing is written there)
+    partial = dgamma if rows == 1 else torch.empty(rows, 2, saved.c_real, dtype=torch.float32, device=dev)
+  _launch(gz, (saved.snap, xr, zr, dgamma, dbeta) + (kept.tensors() if kept else ()), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(),
+          gps, ptr(xr), xps, *(kept.addresses() if kept else (0, 0)), ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c,
           saved.c_real, saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
           ptr(dbeta) if want_affine else 0, int(bool(accumulate)))
   return gx, dgamma if want_affine else None, dbeta if want_affine else None
@@ -916,7 +963,7 @@ def conv_wgrad(layer, x0, x1, gy, accumulate=True):
       with _Timed('act8_wgrad', 2.0 * gy.shape[0] * gy.shape[1] * gy.shape[2] * layer.cout * layer.cin):
         act8_wgrad(x0, gy, layer.cout, layer.cin, db is not None, dw, db, accumulate and acc)
 
-    return _issue_wgrad(layer, (x0.q, x0.s, gy), launch8)
+    return _issue_wgrad(layer, x0.tensors() + (gy,), launch8)
   x0, x1 = [act8_restore(t) if isinstance(t, Act8) else t for t in (x0, x1)]
   x0 = as_nhwc(x0)
   b, h, w, c0 = x0.shape
@@ -1163,7 +1210,7 @@ def _save_conv_inputs(ctx, layer, w_req, x0, x1, *rest):
   if layer.keep8 and w_req:
     kept = [None if t is None else act8_save(t) for t in (x0, x1)]
     ctx.kept = [None if a is None else (a.shape, a.dtype) for a in kept]
-    ctx.save_for_backward(*([t for a in kept for t in ((None, None) if a is None else (a.q, a.s))] + list(rest)))
+    ctx.save_for_backward(*([None if a is None else a.buf for a in kept] + list(rest)))
   else:
     ctx.save_for_backward(x0, x1, *rest)
 
@@ -1173,8 +1220,8 @@ def _saved_conv_inputs(ctx):
   kept = getattr(ctx, 'kept', None)
   if kept is None:
     return saved
-  x = [None if m is None else Act8(saved[2 * i], saved[2 * i + 1], *m) for i, m in enumerate(kept)]
-  return tuple(x) + tuple(saved[4:])
+  x = [None if m is None else Act8._of(b, *m) for b, m in zip(saved, kept)]
+  return tuple(x) + tuple(saved[2:])
 
 
 class ConvAct(torch.autograd.Function):
@@ -1688,7 +1735,7 @@ class LayerNormAct(torch.autograd.Function):
     ctx.meta = (sv.shape, sv.dtype, sv.c_real, sv.eps, sv.slope)
     ctx.keep8 = bool(keep8)
     if keep8:
-      ctx.save_for_backward(sv.kept.q, sv.kept.s, sv.stats, sv.snap, z if slope != 1.0 else None)
+      ctx.save_for_backward(sv.kept.buf, sv.stats, sv.snap, z if slope != 1.0 else None)
     else:
       ctx.save_for_backward(sv.x, sv.snap)
     return z
@@ -1697,8 +1744,8 @@ class LayerNormAct(torch.autograd.Function):
   def backward(ctx, gz):
     z = None
     if ctx.keep8:
-      q, s, stats, snap, z = ctx.saved_tensors
-      sv = LNSaved(None, Act8(q, s, ctx.meta[0], ctx.meta[1]), stats, snap, *ctx.meta)
+      buf, stats, snap, z = ctx.saved_tensors
+      sv = LNSaved(None, Act8._of(buf, ctx.meta[0], ctx.meta[1]), stats, snap, *ctx.meta)
     else:
       x, snap = ctx.saved_tensors
       sv = LNSaved(x, None, None, snap, *ctx.meta)

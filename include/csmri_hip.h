@@ -659,7 +659,8 @@ int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z, int z_pix_
  * forward's stats; with the kept form and slope != 1, z is needed for the sign of y, which it has where slope >= 0
  * (E_ARG below); optional otherwise.  dx may be
  * NULL; dgamma and dbeta (both or neither, [C_real], added to where accumulate != 0) need partial:
- * [csmri_ln_bwd_rows(npix, C)][2][C_real] fp32.  Fixed summation order. */
+ * [csmri_ln_bwd_rows(npix, C)][2][C_real] fp32, or any address where that is one row, which is not written.  Fixed
+ * summation order. */
 int csmri_ln_bwd_rows(long long npix, int C);
 int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const void* x, int x_pix_stride, const void* q8,
                  const uint8_t* s8, const float* stats, const void* z, int z_pix_stride, void* dx, int dx_pix_stride,
