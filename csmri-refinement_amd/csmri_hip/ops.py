@@ -689,10 +689,10 @@ def mx4_linear(x, w, bias=None, slope=1.0, out_dtype=None):
 
 class LNSaved(object):
   """What layer_norm_bwd reads: the input itself or its kept form with the forward's statistics, and the affine
-  parameters as the forward used them."""
+  parameters as the forward used them (``aux``: gamma, beta [2, C], then mean, 1 / std [2, pixels] where x was kept)."""
 
-  def __init__(self, x, kept, stats, snap, shape, dtype, c_real, eps, slope):
-    self.x, self.kept, self.stats, self.snap = x, kept, stats, snap
+  def __init__(self, x, kept, aux, shape, dtype, c_real, eps, slope):
+    self.x, self.kept, self.aux = x, kept, aux
     self.shape, self.dtype, self.c_real, self.eps, self.slope = shape, dtype, c_real, eps, slope
 
 
@@ -703,16 +703,16 @@ def layer_norm(x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
   xr, n, c, ps = _pixels(x)
   if keep8 and slope < 0:
     raise ValueError('csmri_hip: layer_norm with keep8 needs a slope of 0 or more (the backward pass reads the sign of z)')
-  c_real, eps, slope = gamma.shape[0], float(eps), float(slope)
+  c_real, eps, slope = gamma.numel(), float(eps), float(slope)
   gamma, beta = _vector(gamma, c_real, 'gamma'), _vector(beta, c_real, 'beta')
   dev = x.device
   z = torch.empty(x.shape, dtype=x.dtype, device=dev)
-  snap = torch.empty(2, c, dtype=torch.float32, device=dev)
   kept = Act8._new(x) if keep8 else None
-  stats = torch.empty(2, n, dtype=torch.float32, device=dev) if keep8 else None
+  aux = torch.empty(2 * (c + n) if keep8 else 2 * c, dtype=torch.float32, device=dev)
+  snap = aux.data_ptr()
   _launch(x, (gamma, beta), 'csmri_ln_fwd', dt_of(xr), xr.data_ptr(), ps, z.data_ptr(), c, n, c, c_real, gamma.data_ptr(),
-          beta.data_ptr(), eps, slope, snap.data_ptr(), ptr(stats), *(kept.addresses() if keep8 else (0, 0)))
-  return z, LNSaved(None if keep8 else xr, kept, stats, snap, x.shape, x.dtype, c_real, eps, slope)
+          beta.data_ptr(), eps, slope, snap, *((snap + 8 * c,) + kept.addresses() if keep8 else (0, 0, 0)))
+  return z, LNSaved(None if keep8 else xr, kept, aux, x.shape, x.dtype, c_real, eps, slope)
 
 
 def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None, dbeta=None, accumulate=False):
@@ -745,9 +745,10 @@ def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None
                                    torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
     rows = lib.raw('csmri_ln_bwd_rows')(n, c)        # (one: nothing is written there)
     partial = dgamma if rows == 1 else torch.empty(rows, 2, saved.c_real, dtype=torch.float32, device=dev)
-  _launch(gz, (saved.snap, xr, zr, dgamma, dbeta) + (kept.tensors() if kept else ()), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(),
-          gps, ptr(xr), xps, *(kept.addresses() if kept else (0, 0)), ptr(saved.stats), ptr(zr), zps, ptr(gx), c, n, c,
-          saved.c_real, saved.snap.data_ptr(), saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
+  snap = saved.aux.data_ptr()
+  _launch(gz, (saved.aux, xr, zr, dgamma, dbeta) + (kept.tensors() if kept else ()), 'csmri_ln_bwd', dt_of(gr), gr.data_ptr(),
+          gps, ptr(xr), xps, *(kept.addresses() + (snap + 8 * c,) if kept else (0, 0, 0)), ptr(zr), zps, ptr(gx), c, n, c,
+          saved.c_real, snap, saved.eps, saved.slope, ptr(partial), ptr(dgamma) if want_affine else 0,
           ptr(dbeta) if want_affine else 0, int(bool(accumulate)))
   return gx, dgamma if want_affine else None, dbeta if want_affine else None
 
@@ -1735,20 +1736,20 @@ class LayerNormAct(torch.autograd.Function):
     ctx.meta = (sv.shape, sv.dtype, sv.c_real, sv.eps, sv.slope)
     ctx.keep8 = bool(keep8)
     if keep8:
-      ctx.save_for_backward(sv.kept.buf, sv.stats, sv.snap, z if slope != 1.0 else None)
+      ctx.save_for_backward(sv.kept.buf, sv.aux, z if slope != 1.0 else None)
     else:
-      ctx.save_for_backward(sv.x, sv.snap)
+      ctx.save_for_backward(sv.x, sv.aux)
     return z
 
   @staticmethod
   def backward(ctx, gz):
     z = None
     if ctx.keep8:
-      buf, stats, snap, z = ctx.saved_tensors
-      sv = LNSaved(None, Act8._of(buf, ctx.meta[0], ctx.meta[1]), stats, snap, *ctx.meta)
+      buf, aux, z = ctx.saved_tensors
+      sv = LNSaved(None, Act8._of(buf, ctx.meta[0], ctx.meta[1]), aux, *ctx.meta)
     else:
-      x, snap = ctx.saved_tensors
-      sv = LNSaved(x, None, None, snap, *ctx.meta)
+      x, aux = ctx.saved_tensors
+      sv = LNSaved(x, None, aux, *ctx.meta)
     if gz.dtype != sv.dtype:
       gz = gz.to(sv.dtype)
     want = any(ctx.affine_req)
