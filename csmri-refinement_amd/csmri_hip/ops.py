@@ -594,20 +594,23 @@ class Mx4(object):
 
   def __init__(self, codes, scales, k, shape=None):
     cb, sb = 64 * ((k + 127) // 128), 16 * ((k + 511) // 512)        # csmri_mx4_code_bytes, csmri_mx4_scale_bytes
-    for t, nb, what in ((codes, cb, 'codes'), (scales, sb, 'scales')):
-      if t.dtype != torch.uint8 or t.dim() != 2 or t.shape[1] != nb or t.shape[0] != codes.shape[0]:
-        raise ValueError('csmri_hip: 4-bit %s of %d channels have to be uint8 [rows, %d], got %s %s' %
-                         (what, k, nb, t.dtype, tuple(t.shape)))
-      if not t.is_contiguous() or t.data_ptr() % 16:
-        raise ValueError('csmri_hip: 4-bit %s have to be contiguous and 16-byte aligned' % what)
+    rows, u8 = codes.shape[0] if codes.dim() else 0, torch.uint8
+    if codes.dtype != u8 or scales.dtype != u8 or codes.shape != (rows, cb) or scales.shape != (rows, sb):
+      raise ValueError('csmri_hip: 4-bit rows of %d channels are uint8 codes [rows, %d] and scales [rows, %d], got %s %s and %s %s' %
+                       (k, cb, sb, codes.dtype, tuple(codes.shape), scales.dtype, tuple(scales.shape)))
+    if not (codes.is_contiguous() and scales.is_contiguous()) or (codes.data_ptr() | scales.data_ptr()) & 15:
+      raise ValueError('csmri_hip: 4-bit codes and scales have to be contiguous and 16-byte aligned')
     if k <= 0 or k % 8:
       raise ValueError('csmri_hip: 4-bit rows hold a multiple of 8 channels, got %d' % k)
     if codes.get_device() != scales.get_device():
       raise RuntimeError('csmri_hip: operands on %s and %s' % (codes.device, scales.device))
-    self.buf, self._codes, self._scales, self.rows, self.k = None, codes, scales, codes.shape[0], k
-    self.shape = (self.rows, k) if shape is None else tuple(shape)
-    if not self.shape or self.shape[-1] != k or math.prod(self.shape) != self.rows * k:
-      raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (self.rows, self.shape))
+    self.buf, self._codes, self._scales, self.rows, self.k = None, codes, scales, rows, k
+    if shape is None:
+      self.shape = (rows, k)
+    else:
+      self.shape = tuple(shape)
+      if not self.shape or self.shape[-1] != k or math.prod(self.shape) != rows * k:
+        raise ValueError('csmri_hip: 4-bit codes of %d rows for a tensor of %s' % (rows, self.shape))
 
   @classmethod
   def _new(cls, x):
