@@ -340,6 +340,36 @@ def test_layer_norm_strides_accumulation_and_parts(ops):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('keep8', [False, True], ids=['x', 'keep8'])
+@pytest.mark.parametrize('n,c,c_real', [(5, 32, 13), (130, 64, 1), (7, 1040, 520), (3, 4104, 100), (9, 136, 128)])
+def test_layer_norm_of_fewer_channels_than_the_pixels_hold(ops, n, c, c_real, keep8):
+  """Whole vectors of pad channels: the results are those of the pixels cut to their real ones."""
+  x, gz = pixels(n, c, torch.bfloat16, n + c, c_real=c_real), pixels(n, c, torch.bfloat16, n + c + 1, c_real=c_real)
+  cut = pad8(c_real)
+  gamma, beta = torch.rand(c_real, generator=torch.Generator().manual_seed(1)).cuda() + 0.5, torch.full((c_real,), 0.1).cuda()
+  z, sv = ops.layer_norm(x.cuda(), gamma, beta, slope=0.2, keep8=keep8)
+  gx, dg, db = ops.layer_norm_bwd(gz.cuda(), sv, z)
+  assert not z[:, c_real:].any() and not gx[:, c_real:].any()
+  ref, h, mean, r = B.layer_norm(x[:, :c_real], gamma.cpu(), beta.cpu(), 1e-5, 0.2)
+  dh = ln_bounds(x[:, :c_real], gamma.cpu(), 1e-5)
+  g64, s = gamma.cpu().double(), half_step(torch.bfloat16)
+  close(z[:, :c_real], ref, s * ref.abs() + g64 * dh + 4 * U * (h * g64).abs() + 4 * U * 0.1, 'z')
+  # the narrower pixels take other lanes, so their sums differ by roundings: both are within the bound of the exact sums
+  z1, sv1 = ops.layer_norm(x[:, :cut].contiguous().cuda(), gamma, beta, slope=0.2, keep8=keep8)
+  close(z1[:, :c_real], ref, s * ref.abs() + g64 * dh + 4 * U * (h * g64).abs() + 4 * U * 0.1, 'z of the cut pixels')
+  if keep8:
+    h = (B.act8(x)[:, :c_real] - mean) * r
+  gate = torch.where(z[:, :c_real].float().cpu() > 0, 1.0, 0.2).double()
+  rgx, rdg, rdb = B.layer_norm_bwd(gz[:, :c_real], h, r, gate, gamma.cpu())
+  gg = (gz[:, :c_real].double() * gate).abs()
+  t, m1 = gg * g64, lambda v: v.mean(1, keepdim=True)
+  tol = r * (64 * U * (t + m1(t) + 2 * h.abs() * m1(t * h.abs())) + dh * m1(t * h.abs()) + h.abs() * m1(t * dh)) + 64 * U * rgx.abs()
+  close(gx[:, :c_real], rgx, s * rgx.abs() + tol, 'gx')
+  close(dg, rdg, 65 * U * (gg * h.abs()).sum(0) + (gg * dh).sum(0), 'dgamma')
+  close(db, rdb, 65 * U * gg.sum(0), 'dbeta')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('n', [1, 64, 128, 129])
 def test_layer_norm_few_rows_accumulate(ops, n):
   """One workgroup writes the affine gradients itself, several through partial rows: either adds where asked to."""
@@ -369,7 +399,7 @@ def test_layer_norm_large_offset_and_nonfinite_rows(ops):
   close(z[keep], ref, U * ref.abs() + ln_bounds(x[keep], one, 0.0), 'offset')
 
 
-WGRAD_SIZES = [(1, 8, 8), (31, 8, 24), (33, 40, 1), (700, 72, 136), (2048, 64, 64), (5000, 16, 200), (300, 264, 129), (4099, 128, 72)]
+WGRAD_SIZES = [(1, 8, 8), (31, 8, 24), (33, 40, 1), (700, 72, 136), (2048, 64, 64), (5000, 16, 200), (300, 264, 129), (4099, 128, 72), (1030, 72, 264)]
 
 
 @pytest.mark.gpu
@@ -397,6 +427,20 @@ def test_weight_gradient_from_kept_activations(ops, n, cin, cout, dtype):
   assert torch.equal(w0, dw + 3) and torch.equal(b0, db - 2)
   w1, none = ops.act8_wgrad(a, gy.cuda(), cout, cin_real, want_bias=False)
   assert none is None and torch.equal(w1, dw)
+
+
+@pytest.mark.gpu
+def test_weight_gradient_of_many_pixels_and_wide_layers(ops):
+  """Large tiles (256 a side), ragged in both directions and in pixels."""
+  n, cin, cout = 98304 + 77, 264, 300
+  x, gy = pixels(n, cin, torch.bfloat16, 5), pixels(n, pad8(cout), torch.bfloat16, 6, 0.1, 0.0, cout)
+  a = ops.act8_save(x.cuda())
+  dw, db = ops.act8_wgrad(a, gy.cuda(), cout, cin)
+  xr, g = B.act8(x), gy.double()[:, :cout]
+  splits = ops.lib.raw('csmri_act8_wgrad_splits')(ops.dt_of(gy), n, pad8(cout), cin)
+  L = 2 * (n / splits / 32 + 1 + 32) + splits / 64 + 8
+  close(dw, g.t() @ xr, (L + 1) * U * (g.abs().t() @ xr.abs()), 'dw')
+  close(db, g.sum(0), (L + 1) * U * g.abs().sum(0), 'db')
 
 
 @pytest.mark.gpu
