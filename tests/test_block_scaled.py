@@ -159,6 +159,14 @@ def test_weight_gradient_refuses_rows_beyond_32_bit_offsets():
   assert wg(0, p, 1 << 25, p, p, 64, 16, 16, 16, 16, 1, None, p, None, 0, None) == -2
 
 
+def test_4bit_rows_beyond_their_length_are_refused():
+  import csmri_hip
+  raw, p, k = csmri_hip.lib.raw, 1 << 20, (1 << 24) + 8
+  assert raw('csmri_mx4_quantize')(1, p, k, 4, k, p, p, None) == -1
+  assert raw('csmri_mx4_dequantize')(p, p, 4, k, 1, p, k, None) == -1
+  assert raw('csmri_mx4_linear')(4, p, 0, p, 400, k, p, p, 24, None, 1.0, p, 1, 24, p, None) == -1
+
+
 def test_layer_norm_backward_refuses_the_sign_of_z_under_a_negative_slope():
   import csmri_hip
   bw = csmri_hip.lib.raw('csmri_ln_bwd')
@@ -827,3 +835,37 @@ def test_captured_forward_follows_loaded_weights(ops):
       graph.replay()
       assert torch.equal(y, want)
       torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_tensors_beyond_32_bit_offsets(ops):
+  """2^31 elements and more: the last rows come out as they do alone."""
+  n, c, tail = 34000001, 64, 1000
+  x = torch.empty(n, c, dtype=torch.bfloat16, device='cuda')
+  for part in x.split(4000000):
+    part.normal_()
+  last = x[-tail:].clone()
+  gamma, beta = torch.rand(c, device='cuda') + 0.5, torch.rand(c, device='cuda')
+  z, sv = ops.layer_norm(x, gamma, beta, slope=0.2, keep8=True)
+  z1, sv1 = ops.layer_norm(last, gamma, beta, slope=0.2, keep8=True)
+  assert torch.equal(z[-tail:], z1)
+  gz = torch.zeros_like(x)
+  gz[-tail:] = last.flip(0)
+  gx, dg, db = ops.layer_norm_bwd(gz, sv, z)
+  gx1, dg1, db1 = ops.layer_norm_bwd(gz[-tail:], sv1, z1)
+  assert torch.equal(gx[-tail:], gx1) and not gx[:1000].any()
+  # the same terms in another order, and zeros
+  h = ((last.double() - last.double().mean(1, keepdim=True)) / last.double().std(1, keepdim=True)).abs()
+  for a, b, mag in ((dg, dg1, (gz[-tail:].double().abs() * h * 1.2).sum(0)), (db, db1, gz[-tail:].double().abs().sum(0))):
+    assert ((a - b).double().abs() <= 2 * (64 + tail) * U * mag).all()
+  del gx, z
+  assert torch.equal(ops.act8_restore(sv.kept)[-tail:], ops.act8_restore(sv1.kept))
+  dw, _ = ops.act8_wgrad(sv.kept, gz[:, :8])
+  dw1, _ = ops.act8_wgrad(sv1.kept, gz[-tail:, :8].contiguous())
+  mag = gz[-tail:, :8].double().abs().t() @ ops.act8_restore(sv1.kept).double().abs()
+  assert ((dw - dw1).double().abs() <= 2 * (64 + tail) * 2 * U * mag).all()
+  del sv, gz
+  w = ops.mx4_quantize(torch.randn(16, c, device='cuda'))
+  q = ops.mx4_quantize(x)
+  assert torch.equal(ops.mx4_dequantize(q)[-tail:], ops.mx4_dequantize(ops.mx4_quantize(last)))
+  assert torch.equal(ops.mx4_linear(q, w)[-tail:], ops.mx4_linear(last, w))
