@@ -205,8 +205,9 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
 // time.  Both operands pass through registers into one of two LDS stages, the input's codes becoming bf16 on the way, and
 // are loaded a step ahead of that.  (LDS-DMA would spare dY the registers, but the compiler lets no transposed read pass a
 // pending one; a second set of registers, to load two steps ahead, costs more in occupancy than it hides.)  Bound by the
-// matrix unit and the staging beside it: 165 - 177 us at 2048 x 2048 channels and 16384 pixels (800 TFLOP/s), where a loop
-// of products and barriers alone takes 120 - 132.  LDS is not what bounds it: images turned over in
+// matrix unit and the staging beside it: 165 - 177 us at 2048 x 2048 channels and 16384 pixels (800 TFLOP/s), where
+// the products alone take 109 at the clock they leave the chip, their fragment reads and barriers 20 - 28 more, and the loads
+// and staging the rest.  LDS is not what bounds it: images turned over in
 // registers, [channel][pixel], and read 16 bytes at a time halve its reads and took 178.
 //
 // GK = 2: a second set of waves takes every other step, with stages of its own, and hands its sums over at the end -- the
