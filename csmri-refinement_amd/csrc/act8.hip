@@ -414,14 +414,15 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
   }
 }
 
-// Tile: 64 or 128 a side by the channel counts; 256 x 256 (an fp32 dY's three planes do not fit it),
-// which reads LDS a third less per product, where 2048 pixels a split still leave three quarters of the CUs a workgroup.
-// 2048 x 2048 channels, 16384 pixels, with the partial sums: 189 us against 225 with 128 x 128; 512 x 512, 8192 pixels:
-// 46 against 30.
+// Tile: 64 or 128 a side by the channel counts; 256 x 256 (an fp32 dY's three planes do not fit it), which reads LDS a third
+// less per product, where that leaves every CU 2304 pixels of a tile or more -- below, its larger partial sums cost as much
+// -- and covers no more than a tenth beyond what the smaller tiles do.
+// us with it and with 128 x 128, sums included: 16384 pixels, 2048 to 2048 184 / 199; 32768, 1024 to 2048 169 / 194;
+// 16384, 1536 to 1536 110 / 168; 65536, 512 to 1024 101 / 102; 24576, 1024 to 1024 84 / 79; 8192, 2048 to 2048 102 / 99.
 struct A8WTile { int bn, bc; };
 static A8WTile a8w_tile(int dy_dtype, long long npix, int Cout, int Cin) {
-  if (dy_dtype == CSMRI_BF16 && Cout > 128 && Cin > 128 &&
-      (long long)cdiv(Cout, 256) * cdiv(Cin, 256) * (npix / 2048) >= 192) return {256, 256};
+  const double big = (double)cdiv(Cout, 256) * cdiv(Cin, 256), small = (double)cdiv(Cout, 128) * cdiv(Cin, 128);
+  if (dy_dtype == CSMRI_BF16 && big * npix >= 2304. * 256 && 4 * big <= 1.1 * small) return {256, 256};
   return {Cout <= 64 ? 64 : 128, Cin <= 64 ? 64 : 128};
 }
 extern "C" int csmri_act8_wgrad_splits(int dy_dtype, long long npix, int Cout, int Cin) {

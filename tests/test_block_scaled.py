@@ -440,7 +440,7 @@ def test_weight_gradient_from_kept_activations(ops, n, cin, cout, dtype):
 @pytest.mark.gpu
 def test_weight_gradient_of_many_pixels_and_wide_layers(ops):
   """Large tiles (256 a side), ragged in both directions and in pixels."""
-  n, cin, cout = 98304 + 77, 264, 300
+  n, cin, cout = 147456 + 77, 504, 500
   x, gy = pixels(n, cin, torch.bfloat16, 5), pixels(n, pad8(cout), torch.bfloat16, 6, 0.1, 0.0, cout)
   a = ops.act8_save(x.cuda())
   dw, db = ops.act8_wgrad(a, gy.cuda(), cout, cin)
