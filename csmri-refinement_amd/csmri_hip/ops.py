@@ -446,14 +446,17 @@ def _pixels(t):
   if t.is_contiguous():
     ps, ok = c, True
   else:
-    ps, span, ok = c, 0, t.stride(-1) == 1
+    # one stride over all pixels: every axis continues the one inside it.  A broadcast axis (stride 0) continues nothing,
+    # and as the innermost it is a pixel stride that holds no pixel: both are copied
+    ps, span, ok = None, 0, t.stride(-1) == 1
     for size, st in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
       if size == 1 or n == 0:
         continue
-      if span == 0:
+      if ps is None:
         ps, span = st, st * size
       else:
         ok, span = ok and st == span, span * size
+    ps = c if ps is None else ps
     ok = ok and c <= ps < 2 ** 31 and ps * t.element_size() % 16 == 0
   if not ok or t.data_ptr() % 16:
     t, ps = t.contiguous(), c

@@ -1,0 +1,108 @@
+"""Layer norm, 8-bit kept activations and 4-bit products where layouts, devices and values leave the ordinary: broadcast
+pixels, host tensors, buffers that meet, foreign codes, ends of the fp32 range.  The oracle is
+oracle/csmri_blockscale.py, in float64; bounds count roundings like tests/test_block_scaled.py does (u = 2^-24, half a
+step of fp32)."""
+import pytest
+import torch
+
+import csmri_blockscale as B
+
+U = 2.0 ** -24
+
+
+def half_step(dtype):
+  return torch.finfo(dtype).eps / 2
+
+
+def close(got, ref, tol, what=''):
+  got, ref, tol = got.double().cpu(), ref.double().cpu(), tol.double().cpu()
+  bad = ~((got - ref).abs() <= tol)
+  assert not bad.any(), '%s: %d of %d off, worst %.3g over its bound' % (
+      what, int(bad.sum()), bad.numel(), float(((got - ref).abs() / tol.clamp(min=1e-300)).nan_to_num(1e9).max()))
+
+
+@pytest.fixture
+def host_ops(monkeypatch):
+  """csmri_hip.ops for tests that stop short of a launch."""
+  import csmri_hip
+  return csmri_hip.ops
+
+
+@pytest.fixture(scope='module')
+def ops():
+  import csmri_hip
+  assert torch.cuda.is_available()
+  return csmri_hip.ops
+
+
+# ---- broadcast pixels --------------------------------------------------------------------------------------------------
+def layouts(base):
+  """(name, tensor [4, 8, 16, 32] or smaller) for a base [4, 8, 16, 32]: broadcast along every set of pixel axes, and views
+  whose pixels do or do not lie at one stride."""
+  for axes in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2), (0, 1, 2)):
+    t = base
+    for a in axes:
+      t = t.narrow(a, 1, 1)
+    yield 'broadcast %s' % (axes,), t.expand(base.shape)
+    yield 'dense, broadcast %s' % (axes,), t.contiguous().expand(base.shape)
+    yield 'batch of one, broadcast %s' % (axes,), t.contiguous().expand(base.shape)[:1]
+  yield 'dense', base
+  yield 'broadcast channels', base[..., :1].expand(base.shape)
+  yield 'channels', base[..., 8:24]
+  yield 'every other pixel', base[:, :, ::2]
+  yield 'every other row', base[:, ::2]
+  yield 'permuted', base.permute(2, 0, 1, 3)
+  yield 'windows', base.flatten()[:512].as_strided((3, 32), (8, 1))
+  yield 'strided channels', base[..., ::2]
+  yield 'one pixel', base[:1, :1, :1]
+  yield 'no pixel', base[:, :0]
+
+
+def test_pixels_are_read_where_they_lie_or_copied(host_ops, monkeypatch):
+  """What a kernel is given -- an address, a pixel count, a pixel stride -- names the tensor's own values, inside its
+  storage, for any layout."""
+  monkeypatch.setattr(host_ops, '_need_gpu', lambda t: None)
+  base = torch.arange(4 * 8 * 16 * 32, dtype=torch.float32).view(4, 8, 16, 32)
+  for name, t in layouts(base):
+    r, n, c, ps = host_ops._pixels(t)
+    assert n * c == t.numel() and c == t.shape[-1], name
+    if n == 0:
+      continue
+    assert ps >= c and r.storage_offset() + (n - 1) * ps + c <= r.untyped_storage().nbytes() // 4, (name, tuple(t.stride()), ps)
+    assert torch.equal(r.as_strided((n, c), (ps, 1)), t.reshape(n, c)), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('keep8', [False, True], ids=['x', 'keep8'])
+def test_layer_norm_behind_a_pooled_output(ops, keep8):
+  """The gradient that sums over pixels send back is broadcast along the pixel axes."""
+  x = torch.randn(4, 8, 16, 32, generator=torch.Generator().manual_seed(1))
+  gamma, beta = torch.linspace(0.5, 1.5, 32), torch.linspace(-0.3, 0.3, 32)
+  for dims in ((1, 2), (2,), (0, 1, 2)):
+    xd = x.cuda().requires_grad_(True)
+    ga, be = torch.nn.Parameter(gamma.cuda()), torch.nn.Parameter(beta.cuda())
+    z = ops.LayerNormAct.apply(xd, ga, be, 1e-5, 1.0, keep8)
+    s = z.sum(dim=dims)
+    w = torch.randn(s.shape, generator=torch.Generator().manual_seed(2)).cuda()
+    (s * w).sum().backward()
+    g = w.view([1 if i in dims else x.shape[i] for i in range(4)]).expand(x.shape).contiguous()
+    got = ops.layer_norm_bwd(g, ops.layer_norm(xd.detach(), ga.detach(), be.detach(), 1e-5, 1.0, keep8)[1])
+    for a, b in zip((xd.grad, ga.grad, be.grad), got):
+      assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_broadcast_pixels_through_every_operator(ops):
+  base = torch.randn(4, 8, 16, 32, generator=torch.Generator().manual_seed(3)).cuda()
+  w = ops.mx4_quantize(torch.randn(24, 32, generator=torch.Generator().manual_seed(4)).cuda())
+  kept = ops.act8_save(base)
+  gamma, beta = torch.ones(32, device='cuda'), torch.zeros(32, device='cuda')
+  for name, t in layouts(base):
+    if t.shape != base.shape:
+      continue
+    d = t.clone(memory_format=torch.contiguous_format)
+    assert torch.equal(ops.act8_restore(ops.act8_save(t)), ops.act8_restore(ops.act8_save(d))), name
+    assert torch.equal(ops.mx4_linear(t, w), ops.mx4_linear(d, w)), name
+    assert torch.equal(ops.layer_norm(t, gamma, beta)[0], ops.layer_norm(d, gamma, beta)[0]), name
+    for a, b in zip(ops.act8_wgrad(kept, t), ops.act8_wgrad(kept, d)):
+      assert torch.equal(a, b), name
