@@ -467,6 +467,7 @@ def _pixels(t):
 
 def _launch(t, operands, name, *args):
   """lib.call on the current stream of ``t``'s device, where all ``operands`` (None: absent) have to live."""
+  _need_gpu(t)                      # (tensors on the host have one "device" too, -1)
   dev = t.get_device()
   for o in operands:
     if o is not None and o.get_device() != dev:

@@ -106,3 +106,39 @@ def test_broadcast_pixels_through_every_operator(ops):
     assert torch.equal(ops.layer_norm(t, gamma, beta)[0], ops.layer_norm(d, gamma, beta)[0]), name
     for a, b in zip(ops.act8_wgrad(kept, t), ops.act8_wgrad(kept, d)):
       assert torch.equal(a, b), name
+
+
+# ---- tensors on the host -----------------------------------------------------------------------------------------------
+def test_host_operands_reach_no_kernel(host_ops, monkeypatch):
+  """Every operator refuses tensors on the host, whatever device is current."""
+  def launched(name, *args):
+    raise AssertionError('%s would have been launched' % name)
+  monkeypatch.setattr(host_ops.lib, 'call', launched)
+  monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda dev: 0, raising=False)
+  monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: -1, raising=False)
+  o = host_ops
+  z = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+  kept = o.Act8(z(6, 40), z(6, 2), (6, 40), torch.bfloat16)
+  rows, w = o.Mx4(z(6, 128), z(6, 16), 136), o.Mx4(z(24, 128), z(24, 16), 136)
+  x = torch.zeros(6, 40)
+  saved = o.LNSaved(x, None, torch.zeros(80), (6, 40), torch.float32, 40, 1e-5, 1.0)
+  for f in (lambda: o.act8_save(x), lambda: o.act8_restore(kept), lambda: o.act8_restore(kept, torch.float32),
+            lambda: o.act8_wgrad(kept, x), lambda: o.mx4_quantize(torch.zeros(6, 136)), lambda: o.mx4_dequantize(rows),
+            lambda: o.mx4_linear(rows, w), lambda: o.mx4_linear(torch.zeros(6, 136), w),
+            lambda: o.layer_norm(x, torch.ones(40), torch.zeros(40)), lambda: o.layer_norm_bwd(x, saved)):
+    with pytest.raises(RuntimeError):
+      f()
+
+
+@pytest.mark.gpu
+def test_host_operands_beside_device_tensors_are_refused(ops):
+  z = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+  kept, rows = ops.Act8(z(6, 40), z(6, 2), (6, 40), torch.bfloat16), ops.Mx4(z(6, 128), z(6, 16), 136)
+  x = torch.zeros(6, 40, device='cuda')
+  for f in (lambda: ops.act8_restore(kept), lambda: ops.act8_wgrad(kept, x), lambda: ops.mx4_dequantize(rows),
+            lambda: ops.mx4_linear(rows, rows), lambda: ops.mx4_linear(torch.zeros(6, 136, device='cuda'), rows),
+            lambda: ops.mx4_quantize(torch.zeros(6, 136, device='cuda'), rows),
+            lambda: ops.layer_norm(x, torch.ones(40), torch.zeros(40, device='cuda')),
+            lambda: ops.act8_wgrad(ops.act8_save(x), x, dw=torch.zeros(40, 40))):
+    with pytest.raises(RuntimeError):
+      f()
