@@ -968,6 +968,9 @@ def conv_wgrad(layer, x0, x1, gy, accumulate=True):
       LAUNCH_LOG.append(('wgrad', 'act8_wgrad', 1))
 
     def launch8():
+      # this gradient is written at once: what csmri_wgrad has left to reduce for the layer comes before it
+      if any(e[0].dw == dw.data_ptr() for e in _WGRAD['finish']):
+        _finish_wgrads()
       with _Timed('act8_wgrad', 2.0 * gy.shape[0] * gy.shape[1] * gy.shape[2] * layer.cout * layer.cin):
         act8_wgrad(x0, gy, layer.cout, layer.cin, db is not None, dw, db, accumulate and acc)
 

@@ -142,3 +142,44 @@ def test_host_operands_beside_device_tensors_are_refused(ops):
             lambda: ops.act8_wgrad(ops.act8_save(x), x, dw=torch.zeros(40, 40))):
     with pytest.raises(RuntimeError):
       f()
+
+
+# ---- a layer whose gradient comes from two kernels ----------------------------------------------------------------------
+def pointwise_layer(ops, cout, cin, seed, dtype=torch.bfloat16):
+  g = torch.Generator().manual_seed(seed)
+  w = torch.nn.Parameter((torch.randn(cout, cin, 1, 1, generator=g) / cin ** 0.5).cuda())
+  return ops.ConvLayer(w, torch.nn.Parameter(torch.randn(cout, generator=g).cuda()), 1, (0, 0, 0, 0), 'zero', dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('multi', ['0', '1', 'auto'])
+@pytest.mark.parametrize('keeps', [(True, False), (False, True), (False, True, False), (True, False, True)],
+                         ids=lambda k: ''.join('8' if v else '-' for v in k))
+@pytest.mark.parametrize('fresh', [False, True], ids=['accumulate', 'fresh'])
+def test_layer_used_with_kept_and_with_plain_inputs_in_one_backward(ops, monkeypatch, multi, keeps, fresh):
+  """The reductions of plain weight gradients wait for the end of the backward pass: a kept one of the same layer comes
+  after them.  ``fresh``: the gradients hold what a lazy zero left behind, to be overwritten."""
+  monkeypatch.setattr(ops, 'WGRAD_FINISH_MULTI', multi)
+  gen = torch.Generator().manual_seed(7)
+  xs = [torch.randn(2, 24, 20, 40, generator=gen).bfloat16().cuda() for _ in keeps]
+  gs = [(0.1 * torch.randn(2, 24, 20, 24, generator=gen)).bfloat16().cuda() for _ in keeps]
+  layer = pointwise_layer(ops, 24, 40, 3)
+  for p in (layer.weight, layer.bias):
+    p.grad = torch.full_like(p, 7.0)
+    p._grad_fresh = fresh
+  ys = []
+  for x, keep in zip(xs, keeps):
+    layer.keep8 = keep
+    ys.append(ops.ConvAct.apply(x, None, layer.weight, layer.bias, layer, 1.0, None))
+  torch.autograd.backward(ys, gs)
+  base = 0.0 if fresh else 7.0
+  dw = torch.full((24, 40), base, dtype=torch.float64)
+  db = torch.full((24,), base, dtype=torch.float64)
+  mw, mb = dw.abs(), db.abs()
+  for x, g, keep in zip(xs, gs, keeps):
+    x, g = x.double().cpu().view(-1, 40), g.double().cpu().view(-1, 24)
+    x = B.act8(x) if keep else x
+    dw, db, mw, mb = dw + g.t() @ x, db + g.sum(0), mw + g.abs().t() @ x.abs(), mb + g.abs().sum(0)
+  # 960 pixels in products that are exact in fp32: fewer than 100 additions in a chain, each at most 2 u
+  close(layer.weight.grad.view(24, 40), dw, 200 * U * mw, 'dw')
+  close(layer.bias.grad, db, 200 * U * mb, 'db')
