@@ -4,8 +4,8 @@
 //   backward: dy = dz * (y > 0 ? 1 : slope), t = dy gamma,
 //             dx = r (t - mean_c t - h mean_c (t h)), dgamma = sum_p dy h, dbeta = sum_p dy
 //
-// Both passes are bound by HBM: a row is read once into registers, its mean and then its variance around that mean are
-// taken from there (no cancellation, whatever the offset of the data), and written once.  A row of up to 64 lanes x
+// Both passes are bound by HBM: a row is read once into registers, its mean, the deviations' own mean and the variance are
+// taken from there (row_stats: what they cost is relative to the deviations, whatever the offset of the data), and written once.  A row of up to 64 lanes x
 // V vectors of eight channels belongs to one wave -- rows of few channels share a wave -- and a wider one to a
 // workgroup.  The backward recomputes m and r from x with the forward's own arithmetic, so nothing but x is kept; where x
 // itself was kept in 8 bits (micro.h) the forward's m and r are stored next to it and the backward takes 1.03 bytes a
@@ -49,11 +49,16 @@ template <bool WG, int N> __device__ __forceinline__ void row_sums(float (&v)[N]
   }
 }
 
-// mean and 1 / std of U rows held as V vectors a lane; nv[j]: real channels of vector j
+// Statistics of U rows held as V vectors a lane; nv[j]: real channels of vector j.  The rounded mean m0 misses the mean by up
+// to a few steps of an fp32 number of its size, which a row of nearly equal channels would see as a spread of its own.  So x
+// becomes the deviations x - m0 (exact for channels within a factor of two of m0), `corr` their own mean, and
+//   mean = m0 + corr,  h = (x - m0 - corr) inv,  variance = mean (x - m0)^2 - corr^2:
+// errors are relative to the deviations, not to what the row lies around.  (A negative variance, all rounding, counts as 0.)
+// It costs 1 us of a forward and backward of 41 at 8 x 256 x 256 x 32 bf16, with divisions for the products with rc 3.5.
 template <bool WG, int V, int U>
-__device__ __forceinline__ void row_stats(const float (&x)[U][V][8], const int (&nv)[V], const LNParams& p, float (*red)[16],
-                                          int& turn, float (&mean)[U], float (&inv)[U]) {
-  const float rc = 1.f / (float)p.C_real;
+__device__ __forceinline__ void row_stats(float (&x)[U][V][8], const int (&nv)[V], const LNParams& p, float (*red)[16],
+                                          int& turn, float (&m0)[U], float (&corr)[U], float (&inv)[U]) {
+  const float rc = 1.f / (float)p.C_real;       // (rounded too: what it costs m0 is in corr)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float a = 0.f;
@@ -61,22 +66,32 @@ __device__ __forceinline__ void row_stats(const float (&x)[U][V][8], const int (
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int k = 0; k < 8; ++k) a += k < nv[j] ? x[u][j][k] : 0.f;
-    mean[u] = a;
+    m0[u] = a;
   }
-  row_sums<WG, U>(mean, p.group, red, turn);
+  row_sums<WG, U>(m0, p.group, red, turn);
+  float s[2 * U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    mean[u] *= rc;
-    float a = 0.f;
+    m0[u] *= rc;
+    float a = 0.f, b = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) { const float d = k < nv[j] ? x[u][j][k] - mean[u] : 0.f; a = __builtin_fmaf(d, d, a); }
-    inv[u] = a;
+      for (int k = 0; k < 8; ++k) {
+        const float d = k < nv[j] ? x[u][j][k] - m0[u] : 0.f;
+        x[u][j][k] = d;
+        a += d;
+        b = __builtin_fmaf(d, d, b);
+      }
+    s[2 * u] = a; s[2 * u + 1] = b;
   }
-  row_sums<WG, U>(inv, p.group, red, turn);
+  row_sums<WG, 2 * U>(s, p.group, red, turn);
 #pragma unroll
-  for (int u = 0; u < U; ++u) inv[u] = rsqrtf(inv[u] * rc + p.eps);
+  for (int u = 0; u < U; ++u) {
+    corr[u] = s[2 * u] * rc;
+    const float v = __builtin_fmaf(-corr[u], corr[u], s[2 * u + 1] * rc);
+    inv[u] = rsqrtf((v < 0.f ? 0.f : v) + p.eps);
+  }
 }
 
 // the affine step, spelled out so that the forward and the backward's sign test round alike
@@ -128,32 +143,39 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
   const int sblocks = (p.C + MICRO_BLOCK - 1) / MICRO_BLOCK;
   const bool act = p.slope != 1.f;
   for (long long row = first; row - gi < p.rows; row += step * U) {
-    float x[U][V][8], mean[U], inv[U];
+    float x[U][V][8], m0[U], corr[U], inv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < V; ++j) cvt8<DT>(raw[u][j], x[u][j]);
     fetch(row + step * U);                           // the next rows come in under this one's arithmetic
     __builtin_amdgcn_sched_barrier(0);
-    row_stats<WG, V, U>(x, nv, p, red, turn, mean, inv);
+    if constexpr (KEEP) {                            // x itself, before it turns into deviations
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long rr = row + u * step;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {                // all lanes take part in the block's maximum
+          const unsigned amax = block_amax(x[u][j]);
+          unsigned char sc;
+          const u32x2_t o = micro_pack8(x[u][j], amax, sc);
+          if (rr < p.rows && c[j] < p.C) {
+            *(u32x2_t*)(p.qo + rr * p.C + c[j]) = o;
+            if ((c[j] & (MICRO_BLOCK - 1)) == 0) p.so[rr * sblocks + c[j] / MICRO_BLOCK] = sc;
+          }
+        }
+      }
+    }
+    row_stats<WG, V, U>(x, nv, p, red, turn, m0, corr, inv);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const long long rr = row + u * step;
       const bool live = rr < p.rows;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if constexpr (KEEP) {                        // all lanes take part in the block's maximum
-          const unsigned amax = block_amax(x[u][j]);
-          unsigned char sc;
-          const u32x2_t o = micro_pack8(x[u][j], amax, sc);
-          if (live && c[j] < p.C) {
-            *(u32x2_t*)(p.qo + rr * p.C + c[j]) = o;
-            if ((c[j] & (MICRO_BLOCK - 1)) == 0) p.so[rr * sblocks + c[j] / MICRO_BLOCK] = sc;
-          }
-        }
         float o[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = ln_affine((x[u][j][k] - mean[u]) * inv[u], ga[j][k], be[j][k]);
+        for (int k = 0; k < 8; ++k) o[k] = ln_affine((x[u][j][k] - corr[u]) * inv[u], ga[j][k], be[j][k]);
         if (act) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) o[k] = o[k] > 0.f ? o[k] : o[k] * p.slope;
@@ -162,7 +184,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LNParams p) {
         for (int k = 0; k < 8; ++k) o[k] = k < nv[j] ? o[k] : 0.f;
         if (live && c[j] < p.C) st8<DT>(p.out, rr * p.ops + c[j], o);
       }
-      if (live && gl == 0 && p.stats_out) { p.stats_out[rr] = mean[u]; p.stats_out[p.rows + rr] = inv[u]; }
+      if (live && gl == 0 && p.stats_out) { p.stats_out[rr] = m0[u] + corr[u]; p.stats_out[p.rows + rr] = inv[u]; }
     }
   }
 }
@@ -214,7 +236,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) dg[j][k] = db[j][k] = 0.f;
   for (long long row = first; row - gi < p.rows; row += step * U) {
-    float x[U][V][8], t[U][V][8], mean[U], inv[U];
+    float x[U][V][8], t[U][V][8], sub[U], inv[U];     // h = (x - sub) inv
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -222,7 +244,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
         if constexpr (KEPT) micro_unpack8(rq[u][j], micro_scale(rs[u][j]), x[u][j]);
         else cvt8<DT>(rx[u][j], x[u][j]);
         cvt8<DT>(rg[u][j], t[u][j]);
-        if constexpr (KEPT) { mean[u] = rm[u]; inv[u] = ri[u]; }
+        if constexpr (KEPT) { sub[u] = rm[u]; inv[u] = ri[u]; }
       }
     if (gate_z) {
 #pragma unroll
@@ -239,7 +261,8 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
     }
     fetch(row + step * U);                           // the next rows come in under this one's arithmetic
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (!KEPT) row_stats<WG, V, U>(x, nv, p, red, turn, mean, inv);
+    float m0[U];
+    if constexpr (!KEPT) row_stats<WG, V, U>(x, nv, p, red, turn, m0, sub, inv);
     float s[2 * U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -248,7 +271,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LNParams p) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[u][j][k] = (x[u][j][k] - mean[u]) * inv[u];
+        for (int k = 0; k < 8; ++k) x[u][j][k] = (x[u][j][k] - sub[u]) * inv[u];
         if (gate_x) {
 #pragma unroll
           for (int k = 0; k < 8; ++k)

@@ -183,3 +183,89 @@ def test_layer_used_with_kept_and_with_plain_inputs_in_one_backward(ops, monkeyp
   # 960 pixels in products that are exact in fp32: fewer than 100 additions in a chain, each at most 2 u
   close(layer.weight.grad.view(24, 40), dw, 200 * U * mw, 'dw')
   close(layer.bias.grad, db, 200 * U * mb, 'db')
+
+
+# ---- layer norm of rows far from zero ------------------------------------------------------------------------------------
+def ln_offset_bounds(x, eps):
+  """Bounds of |error of h| for the two-step mean: m0 = mean + d0, |d0| <= 66 u mean|x| (chains of fewer than 64 additions,
+  a division); d = x - m0, then mean(d) corrects both the deviations and the variance.  A deviation is off by
+  u |d| + 67 u mean|d| + its own rounding, mean d^2 - mean(d)^2 by 70 u (var + 2 d0^2), 1 / sqrt by half of that relatively
+  and 4 u."""
+  x = x.double()
+  mean = x.mean(1, keepdim=True)
+  var = ((x - mean) ** 2).mean(1, keepdim=True)
+  d0 = 66 * U * x.abs().mean(1, keepdim=True)
+  dev = (x - mean).abs()
+  r = 1 / torch.sqrt(var + eps)
+  dnum = 70 * U * (dev + dev.mean(1, keepdim=True) + 2 * d0)
+  drel = 35 * U * (var + 2 * d0 ** 2) / (var + eps) + 4 * U
+  return r * dnum + (dev * r + r * dnum) * drel + 2 * U * dev * r
+
+
+OFFSET_SIZES = [7, 13, 15, 64, 100, 520, 1000, 2056, 4100, 8190]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('offset', [1000.0, -10000.0])
+@pytest.mark.parametrize('c', OFFSET_SIZES)
+def test_layer_norm_of_constant_rows(ops, c, offset):
+  """Every deviation is zero: z is beta, whatever the mean's sum rounds to."""
+  cp = (c + 7) // 8 * 8
+  for dtype in (torch.float32, torch.bfloat16):
+    x = torch.zeros(5, cp, dtype=dtype)
+    x[:, :c] = offset
+    x[1, :c] = offset * 1.1
+    gamma, beta = torch.linspace(0.5, 1.5, c), torch.linspace(-0.3, 0.3, c)
+    z, saved = ops.layer_norm(x.cuda(), gamma.cuda(), beta.cuda())
+    dh = ln_offset_bounds(x[:, :c], 1e-5)
+    close(z[:, :c], beta.expand(5, c), half_step(dtype) * beta.abs().double() + gamma.double() * dh + 4 * U * beta.abs().double(), 'z')
+    gz = torch.randn(5, cp, generator=torch.Generator().manual_seed(c)).to(dtype)
+    gz[:, c:] = 0
+    gx, dg, db = ops.layer_norm_bwd(gz.cuda(), saved)
+    t = gz[:, :c].double() * gamma.double()
+    ref, r = (t - t.mean(1, keepdim=True)) / 1e-5 ** 0.5, 1e-5 ** -0.5
+    m1 = lambda v: v.mean(1, keepdim=True)
+    close(gx[:, :c], ref, half_step(dtype) * ref.abs() + r * (70 * U * (t.abs() + m1(t.abs())) + dh * m1(t.abs() * dh)) + 64 * U * ref.abs(), 'gx')
+    close(dg, torch.zeros(c), (gz[:, :c].double().abs() * dh).sum(0) + 1e-300, 'dgamma')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('spread', [1.0, 2.0 ** -6, 2.0 ** -10])
+@pytest.mark.parametrize('c', OFFSET_SIZES)
+def test_layer_norm_of_a_small_spread_around_a_large_offset(ops, c, spread):
+  """fp32 rows around 1000 whose spread is a few of their own steps (2^-14) and more: what the statistics cost is relative
+  to the spread, forward and backward."""
+  cp, eps = (c + 7) // 8 * 8, 1e-5
+  g = torch.Generator().manual_seed(c)
+  x = torch.zeros(6, cp)
+  x[:, :c] = 1000 + spread * torch.randn(6, c, generator=g)
+  gz = torch.zeros(6, cp)
+  gz[:, :c] = torch.randn(6, c, generator=g)
+  gamma, beta = torch.linspace(0.5, 1.5, c), torch.linspace(-0.3, 0.3, c)
+  z, saved = ops.layer_norm(x.cuda(), gamma.cuda(), beta.cuda(), eps)
+  ref, h, mean, r = B.layer_norm(x[:, :c], gamma, beta, eps, 1.0)
+  dh = ln_offset_bounds(x[:, :c], eps)
+  g64, b64 = gamma.double(), beta.double()
+  close(z[:, :c], ref, U * ref.abs() + g64 * dh + 4 * U * (h * g64).abs() + 4 * U * b64.abs(), 'z')
+  gx, dg, db = ops.layer_norm_bwd(gz.cuda(), saved)
+  rgx, rdg, rdb = B.layer_norm_bwd(gz[:, :c], h, r, torch.ones_like(h), gamma)
+  t, m1 = gz[:, :c].double().abs() * g64, lambda v: v.mean(1, keepdim=True)
+  h = h.abs()
+  tol = r * (70 * U * (t + m1(t) + 2 * h * m1(t * h)) + dh * m1(t * h) + h * m1(t * dh) + dh * m1(t * dh))
+  # r itself: 35 u (var + 2 d0^2) / (var + eps) + 4 u, at most 110 u with d0 <= 66 u 1000 against eps
+  close(gx[:, :c], rgx, U * rgx.abs() + tol + 110 * U * r * (t + m1(t) + h * m1(t * h)), 'gx')
+  close(dg, rdg, (gz[:, :c].double().abs() * (dh + 64 * U * h)).sum(0) + 1e-300, 'dgamma')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('c', [15, 100, 4100])
+def test_kept_layer_norm_of_constant_rows(ops, c):
+  """The kept form's statistics: the mean of a constant row is its value to one rounding, 1 / std that of eps."""
+  cp = (c + 7) // 8 * 8
+  x = torch.zeros(3, cp)
+  x[:, :c] = torch.tensor([1000.0, -10000.0, 12345.678]).view(3, 1)
+  _, saved = ops.layer_norm(x.cuda(), torch.ones(c).cuda(), torch.zeros(c).cuda(), keep8=True)
+  mean, r = saved.aux[2 * cp:2 * cp + 3].double().cpu(), saved.aux[2 * cp + 3:].double().cpu()
+  ref = x[:, 0].double()
+  close(mean, ref, 2 * U * ref.abs(), 'mean')
+  close(r, torch.full((3,), 1e-5 ** -0.5, dtype=torch.float64), torch.full((3,), 110 * U * 1e-5 ** -0.5, dtype=torch.float64), '1 / std')
