@@ -170,8 +170,8 @@ int micro_colsum2(const float* partial, int rows, long long row_stride, long lon
 // ---- weight gradient of a 1 x 1 convolution ---------------------------------------------------------------------------
 //   dW[n][c] = sum_p dY[p][n] * Xhat[p][c],  db[n] = sum_p dY[p][n]
 // An e4m3 element times its power-of-two scale is a bf16 number exactly, so the kept activations enter
-// v_mfma_f32_16x16x32_bf16 without a rounding of their own; an fp32 dY is split into three bf16 parts whose sum is
-// exact, three products each.  The sum runs over pixels, the strided direction of both operands: LDS images keep
+// v_mfma_f32_16x16x32_bf16 without a rounding of their own; an fp32 dY is split into three bf16 parts (split3), three
+// products each.  The sum runs over pixels, the strided direction of both operands: LDS images keep
 // [pixel][channel] and ds_read_b64_tr_b16 hands out the pixel-contiguous fragments.
 struct A8WParams {
   const char* dy; int dyps;
@@ -182,14 +182,17 @@ struct A8WParams {
   float* dw; float* db; int accumulate;
 };
 
-// three bf16 parts of eight floats: f = h + m + l exactly
+// three bf16 parts of eight floats: f = h + m + l exactly from 2^-103 up (below, the third part is no normal bf16 number any
+// more).  The parts are cut off, not rounded: eight bits each are the 24 of an fp32 number, and h never passes bf16's largest
+// one.  An infinity or a NaN is its first part, the others are zero.
 __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
   float h[8], m[8], l[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    h[k] = (float)(__bf16)f[k];
-    const float r = f[k] - h[k];
-    m[k] = (float)(__bf16)r;
+    const bool finite = abs_bits(f[k]) < 0x7f800000u;
+    h[k] = finite ? __uint_as_float(__float_as_uint(f[k]) & 0xffff0000u) : f[k];
+    const float r = finite ? f[k] - h[k] : 0.f;
+    m[k] = __uint_as_float(__float_as_uint(r) & 0xffff0000u);
     l[k] = r - m[k];
   }
   const float* part[3] = {h, m, l};

@@ -680,7 +680,8 @@ int csmri_act8_restore(const void* q8, const uint8_t* s8, long long npix, int C,
 /* Weight gradient of a 1 x 1 stride-1 convolution whose input was kept in 8 bits (csmri_wgrad for that case):
  *   dw[n][c] (+)= sum_p dy[p][n] xhat[p][c],  db[n] (+)= sum_p dy[p][n]
  * dw: fp32 [Cout_real][Cin_real]; db: fp32 [Cout_real] or NULL; Cout, Cin: padded channel counts of dy and of the kept
- * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts.
+ * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts,
+ * without loss from 2^-103 up.
  * splits: csmri_act8_wgrad_splits; slab: csmri_act8_wgrad_slab_bytes (NULL when that is 0).  Fixed summation order.
  * npix == 0 leaves zeros (or what was there, with accumulate).  64 pixels of dy and of q8 stay below 2^31 bytes
  * (E_UNSUPPORTED otherwise). */

@@ -269,3 +269,43 @@ def test_kept_layer_norm_of_constant_rows(ops, c):
   ref = x[:, 0].double()
   close(mean, ref, 2 * U * ref.abs(), 'mean')
   close(r, torch.full((3,), 1e-5 ** -0.5, dtype=torch.float64), torch.full((3,), 110 * U * 1e-5 ** -0.5, dtype=torch.float64), '1 / std')
+
+
+# ---- the ends of the fp32 range in a gradient that is split into three bf16 parts ------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize('n,cin,cout', [(40, 24, 16), (700, 72, 136)])
+def test_weight_gradient_of_infinite_nan_and_largest_fp32_gradients(ops, n, cin, cout):
+  """An infinity in dY stays one, with the sign of the activation it meets, NaN stays NaN, finite values beyond the largest
+  bf16 number stay finite, and none of them leaves its output channel."""
+  g = torch.Generator().manual_seed(n)
+  x = (torch.rand(n, cin, generator=g) + 0.5) * (1 - 2 * torch.randint(0, 2, (1, cin), generator=g))   # one sign a channel
+  x = x * 2.0 ** -10
+  gy = 0.1 * torch.randn(n, cout, generator=g)
+  top = torch.finfo(torch.float32).max
+  gy[n - 1, 0], gy[3, 1], gy[5, 2] = float('inf'), -float('inf'), float('nan')
+  gy[7, 3], gy[8, 4], gy[9, 5] = 3.4e38, -top, 3.396e38
+  kept = ops.act8_save(x.cuda())
+  xq = B.act8(x)
+  dw, db = [t.double().cpu() for t in ops.act8_wgrad(kept, gy.cuda(), cout, cin)]
+  for row, v in ((0, float('inf')), (1, -float('inf'))):
+    assert torch.equal(dw[row], v * xq[0].sign()) and db[row] == v
+  assert torch.isnan(dw[2]).all() and torch.isnan(db[2])
+  rest = [i for i in range(cout) if i > 2]
+  g64 = gy.double()[:, rest]
+  # three parts of 8 bits each, of one sign: their products are exact, each of at most 6 (n / 32 + 33) additions 2 u
+  L = 6 * (n / 32 + 33) + 8
+  close(dw[rest], g64.t() @ xq, L * U * (g64.abs().t() @ xq.abs()), 'dw')
+  close(db[rest], g64.sum(0), L * U * g64.abs().sum(0), 'db')
+
+
+@pytest.mark.gpu
+def test_weight_gradient_of_small_fp32_gradients(ops):
+  """dY around 2^-100, whose third parts are the smallest that are still normal bf16 numbers: as exact as any other."""
+  g = torch.Generator().manual_seed(5)
+  x, gy = torch.randn(300, 40, generator=g), torch.randn(300, 24, generator=g) * 2.0 ** -98
+  gy = torch.where(gy.abs() < 2.0 ** -103, torch.zeros(()), gy)
+  dw, db = ops.act8_wgrad(ops.act8_save(x.cuda()), gy.cuda())
+  xq, g64 = B.act8(x), gy.double()
+  L = 6 * (300 / 32 + 33) + 8
+  close(dw, g64.t() @ xq, L * U * (g64.abs().t() @ xq.abs()), 'dw')
+  close(db, g64.sum(0), L * U * g64.abs().sum(0), 'db')
