@@ -259,52 +259,52 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
     const int id = j * NT + tid, ch = id % CC;
     xrow[j] = id / CC; xoff[j] = img_off<CC>(xrow[j], ch); xch[j] = c0 + ch * 8 < p.Cin ? c0 + ch * 8 : 0;
   }
-  raw8<DT> yv[2][NY]; u32x2_t xv[2][NX]; unsigned sv[2][NX];
+  raw8<DT> yv[NY]; u32x2_t xv[NX]; unsigned sv[NX];
   auto left_of = [&](int k) { const long long l = pe - pb - (long long)k * KP; return l < KP ? (int)l : KP; };
   // (behind the last step: the last one again, with a dY of zero)
-  auto fetch = [&](int s, int b) {
+  auto fetch = [&](int s) {
     const int k = min(s * GK + part, steps - 1);
     const long long pix = pb + (long long)k * KP;
     const char* yb = p.dy + pix * p.dyps * ES;
     const unsigned char* xb = p.q + pix * p.Cin; const unsigned char* sb = p.s + pix * sblocks;
     const int last = left_of(k) - 1;
 #pragma unroll
-    for (int j = 0; j < NY; ++j) yv[b][j] = ldraw8<DT>(yb + (unsigned)(min(yrow[j], last) * p.dyps * ES + ych[j]), 0);
+    for (int j = 0; j < NY; ++j) yv[j] = ldraw8<DT>(yb + (unsigned)(min(yrow[j], last) * p.dyps * ES + ych[j]), 0);
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
       const int r = min(xrow[j], last);
-      xv[b][j] = *(const u32x2_t*)(xb + (unsigned)(r * p.Cin + xch[j]));
-      sv[b][j] = sb[(unsigned)(r * sblocks + (xch[j] >> 5))];
+      xv[j] = *(const u32x2_t*)(xb + (unsigned)(r * p.Cin + xch[j]));
+      sv[j] = sb[(unsigned)(r * sblocks + (xch[j] >> 5))];
     }
   };
-  auto place = [&](int s, int b) {
+  auto place = [&](int s) {
     char* yi = stages + (s & 1) * STG; char* xi = yi + PL * YIMG;
     const int left = left_of(s * GK + part);
     if (left < KP) {
 #pragma unroll
       for (int j = 0; j < NY; ++j)
-        if (yrow[j] >= left) yv[b][j] = raw8<DT>{};
+        if (yrow[j] >= left) yv[j] = raw8<DT>{};
     }
 #pragma unroll
     for (int j = 0; j < NY; ++j) {
       if constexpr (DT == CSMRI_F32) {
         float f[8]; u32x4_t o[3];
-        cvt8<DT>(yv[b][j], f);
+        cvt8<DT>(yv[j], f);
         split3(f, o);
 #pragma unroll
         for (int i = 0; i < 3; ++i) *(u32x4_t*)(yi + i * YIMG + yoff[j]) = o[i];
       } else {
-        *(u32x4_t*)(yi + yoff[j]) = yv[b][j].a;
+        *(u32x4_t*)(yi + yoff[j]) = yv[j].a;
       }
     }
 #pragma unroll
     for (int j = 0; j < NX; ++j) {
-      const float s = __uint_as_float(sv[b][j] << 23);
+      const float s = __uint_as_float(sv[j] << 23);
       u32x4_t o;
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        o[2 * q] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[b][j][q], s, false));
-        o[2 * q + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[b][j][q], s, true));
+        o[2 * q] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, false));
+        o[2 * q + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xv[j][q], s, true));
       }
       *(u32x4_t*)(xi + xoff[j]) = o;
     }
@@ -350,15 +350,15 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
       }
     };
     if (steps == 0) return;
-    fetch(0, 0);
-    place(0, 0);
-    fetch(1, 0);
+    fetch(0);
+    place(0);
+    fetch(1);
     for (int s = 0; s < mine; ++s) {
       barrier();                                  // stage s is there for everyone; everyone has read stage s - 1
       // half of the waves multiply first, so that staging and products run side by side
       if (wn & 1) { multiply(s); __builtin_amdgcn_sched_barrier(0); }
-      place(s + 1, 0);
-      fetch(s + 2, 0);
+      place(s + 1);
+      fetch(s + 2);
       __builtin_amdgcn_sched_barrier(0);
       if (!(wn & 1)) multiply(s);
     }
