@@ -93,8 +93,10 @@ __device__ __forceinline__ u32x2_t micro_pack8(const float* v, unsigned amax, un
   scale = (unsigned char)(e + 127);
   return q;
 }
-// scale byte -> factor; 255 gives infinity, and the codes of such a block are NaN
-__device__ __forceinline__ float micro_scale(unsigned char s) { return __uint_as_float((unsigned)s << 23); }
+// scale byte -> factor: 0 is 2^-127, no normal fp32 number, and 255 NaN
+__device__ __forceinline__ float micro_scale(unsigned char s) {
+  return __uint_as_float(s == 0 ? 0x00400000u : (s == MICRO_NAN ? 0x7fc00000u : (unsigned)s << 23));
+}
 
 __device__ __forceinline__ void micro_unpack8(u32x2_t q, float s, float* v) {
 #pragma unroll

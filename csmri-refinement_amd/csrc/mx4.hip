@@ -133,8 +133,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const unsigned* __r
     for (int u = 0; u < U; ++u) {
       if (row + u * step >= rows) break;
       float v[8];
-      // scale 1 here: the factor is applied as an fp32 product, exact, and a NaN scale byte becomes a NaN factor
-      const float f = sc[u] == MICRO_NAN ? __uint_as_float(0x7fc00000u) : (sc[u] ? micro_scale(sc[u]) : __uint_as_float(0x00400000u));
+      // scale 1 here: the factor is applied as an fp32 product, exact
+      const float f = micro_scale(sc[u]);
       auto t = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 0); v[0] = t[0] * f; v[1] = t[1] * f;
       t = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 1); v[2] = t[0] * f; v[3] = t[1] * f;
       t = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 2); v[4] = t[0] * f; v[5] = t[1] * f;

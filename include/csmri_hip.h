@@ -671,7 +671,7 @@ int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const void* x, in
  * Activations kept for the backward pass in 8 bits: e4m3fn codes q8 [npix][C] (8-byte aligned, dense) and one E8M0 scale
  * byte per 32 consecutive channels of a pixel, s8 [npix][ceil(C / 32)] (value 2^(s8 - 127)):
  *   e = max(floor(log2(max |x| of the block)), -100), s8 = e - 7 + 127, q8 = e4m3_rne(x / 2^(e - 7))
- * |x / scale| < 256, so nothing saturates.  A block with a NaN or an infinity: s8 = 255, codes NaN, all of it reads NaN.
+ * |x / scale| < 256, so nothing saturates.  A block with a NaN or an infinity: s8 = 255, codes NaN; a block of scale byte 255 reads NaN.
  * C % 8 == 0.  csmri_act8_restore writes the values (exact in either dtype; a magnitude within half a step of 2^128
  * reads as infinity). */
 int csmri_act8_save(int dtype, const void* x, int x_pix_stride, long long npix, int C, void* q8, uint8_t* s8, void* stream);

@@ -309,3 +309,38 @@ def test_weight_gradient_of_small_fp32_gradients(ops):
   L = 6 * (300 / 32 + 33) + 8
   close(dw, g64.t() @ xq, L * U * (g64.abs().t() @ xq.abs()), 'dw')
   close(db, g64.sum(0), L * U * g64.abs().sum(0), 'db')
+
+
+# ---- scale bytes that only codes from elsewhere hold ------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_kept_codes_with_the_smallest_and_the_nan_scale(ops):
+  """Scale byte 0 is 2^-127, 255 is NaN whatever the codes: where the values are restored, in the weight gradient and in
+  the layer norm's backward."""
+  g = torch.Generator().manual_seed(11)
+  code = torch.randint(72, 120, (6, 64), generator=g).to(torch.uint8)      # e4m3 4 .. 240: with 2^-127 a normal number
+  sign = torch.randint(0, 2, (6, 64), generator=g).to(torch.uint8) * 128
+  code = code + sign
+  scale = torch.tensor([0, 1, 254, 127, 0, 100], dtype=torch.uint8).view(6, 1).repeat(1, 2)
+  value = torch.tensor(B.E4M3, dtype=torch.float64)[(code % 128).long()] * torch.where(sign > 0, -1.0, 1.0).double()
+  value = value * torch.exp2(scale.double() - 127).repeat_interleave(32, 1)
+  kept = lambda s: ops.Act8(code.cuda(), s.cuda(), (6, 64), torch.float32)
+  got = ops.act8_restore(kept(scale)).double().cpu()
+  ok = value.abs() < torch.finfo(torch.float32).max
+  assert torch.equal(got[ok], value[ok]) and torch.isinf(got[~ok]).all()
+  nan = scale.clone()
+  nan[3, 1] = 255
+  got = ops.act8_restore(kept(nan)).cpu()
+  assert torch.isnan(got[3, 32:]).all() and int(torch.isnan(got).sum()) == 32
+  assert torch.isnan(ops.act8_wgrad(kept(nan), torch.ones(6, 8, device='cuda'))[0][:, 32:]).all()
+  # one pixel at a time, so that the large ones do not hide the small
+  for p in (0, 1, 4, 5):
+    gy = torch.full((1, 8), 2.0 ** 90)
+    one = ops.Act8(code[p:p + 1].cuda(), scale[p:p + 1].cuda(), (1, 64), torch.float32)
+    for dt in (torch.float32, torch.bfloat16):
+      dw, _ = ops.act8_wgrad(one, gy.to(dt).cuda())
+      assert torch.equal(dw.double().cpu(), value[p:p + 1].mul(2.0 ** 90).expand(8, 64)), (p, dt)
+  x = torch.randn(6, 64, generator=g)
+  z, saved = ops.layer_norm(x.cuda(), torch.ones(64).cuda(), torch.zeros(64).cuda(), keep8=True)
+  saved.kept = kept(nan)
+  gx = ops.layer_norm_bwd(torch.ones(6, 64, device='cuda'), saved, z)[0].cpu()
+  assert torch.isnan(gx[3]).all()
