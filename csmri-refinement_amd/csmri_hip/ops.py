@@ -493,6 +493,13 @@ def _into(t, n, what):
   return t
 
 
+def _apart(a, b, what):
+  """Two fp32 buffers that kernels write have no element in common."""
+  p, q = a.data_ptr(), b.data_ptr()
+  if p < q + 4 * b.numel() and q < p + 4 * a.numel():
+    raise ValueError('csmri_hip: %s share memory' % what)
+
+
 class Act8(object):
   """An activation tensor kept in 8 bits (csmri_act8_save): ``q`` uint8 [pixels, C], ``s`` uint8 [pixels, ceil(C / 32)],
   ``shape`` and ``dtype`` of what was saved."""
@@ -577,7 +584,7 @@ def act8_wgrad(a, gy, cout=None, cin=None, want_bias=True, dw=None, db=None, acc
   if dw is not None:
     _into(dw, cout * cin, 'dw')
     if db is not None:
-      _into(db, cout, 'db')
+      _apart(dw, _into(db, cout, 'db'), 'dw and db')
   elif db is not None:
     raise ValueError('csmri_hip: act8_wgrad writes db only next to a dw')
   else:
@@ -745,8 +752,7 @@ def layer_norm_bwd(gz, saved, z=None, want_x=True, want_affine=True, dgamma=None
     if (dgamma is None) != (dbeta is None):
       raise ValueError('csmri_hip: layer_norm_bwd writes dgamma and dbeta, both or neither')
     if dgamma is not None:
-      _into(dgamma, saved.c_real, 'dgamma')
-      _into(dbeta, saved.c_real, 'dbeta')
+      _apart(_into(dgamma, saved.c_real, 'dgamma'), _into(dbeta, saved.c_real, 'dbeta'), 'dgamma and dbeta')
     else:
       dgamma, dbeta, accumulate = (torch.empty(saved.c_real, dtype=torch.float32, device=dev),
                                    torch.empty(saved.c_real, dtype=torch.float32, device=dev), False)
@@ -1740,6 +1746,8 @@ class LayerNormAct(torch.autograd.Function):
   def forward(ctx, x, gamma, beta, eps=1e-5, slope=1.0, keep8=False):
     if not (gamma.is_leaf and beta.is_leaf):
       raise ValueError('csmri_hip: LayerNormAct writes the gradients of gamma and beta itself: they have to be leaf tensors')
+    if gamma is beta:
+      raise ValueError('csmri_hip: LayerNormAct needs two tensors for gamma and beta: their gradients are written at once')
     z, sv = layer_norm(x, gamma, beta, eps, slope, keep8)
     ctx.gamma, ctx.beta = gamma, beta
     ctx.affine_req = (gamma.requires_grad, beta.requires_grad)

@@ -473,6 +473,7 @@ extern "C" int csmri_act8_wgrad(int dy_dtype, const void* dy, int dy_pix_stride,
   hipStream_t st = (hipStream_t)stream;
   CSMRI_CHECK_ARG(npix == 0 || (dy && q8 && s8));
   CSMRI_CHECK_ARG(splits == 1 || (slab && splits <= npix));
+  CSMRI_CHECK_ARG(!buffers_meet(dw, (long long)Cout_real * Cin_real, db, Cout_real));
   if (npix && (((uintptr_t)dy & 15) || ((uintptr_t)q8 & 7) || ((long long)dy_pix_stride * dtype_size(dy_dtype)) % 16)) return CSMRI_E_ALIGN;
   A8WParams p = {};
   p.dy = (const char*)dy; p.dyps = dy_pix_stride;

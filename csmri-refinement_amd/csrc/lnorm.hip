@@ -449,6 +449,7 @@ extern "C" int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const 
   if (C > LN_MAX_C) return CSMRI_E_UNSUPPORTED;
   hipStream_t st = (hipStream_t)stream;
   if (npix == 0) {
+    CSMRI_CHECK_ARG(!buffers_meet(dgamma, C_real, dbeta, C_real));
     int rc = CSMRI_OK;
     if (dgamma && !accumulate) rc = csmri_fill_f32(dgamma, C_real, 0.f, stream);
     if (rc == CSMRI_OK && dbeta && !accumulate) rc = csmri_fill_f32(dbeta, C_real, 0.f, stream);
@@ -462,6 +463,7 @@ extern "C" int csmri_ln_bwd(int dtype, const void* dz, int dz_pix_stride, const 
   if (!ln_aligned(dz, dz_pix_stride, dtype) || (x && !ln_aligned(x, x_pix_stride, dtype)) ||
       (z && !ln_aligned(z, z_pix_stride, dtype)) || (dx && !ln_aligned(dx, dx_pix_stride, dtype)) ||
       ((uintptr_t)q8 & 7) || ((uintptr_t)affine_snap & 15)) return CSMRI_E_ALIGN;
+  CSMRI_CHECK_ARG(!buffers_meet(dgamma, C_real, dbeta, C_real));
   LNParams p = {};
   p.x = x; p.xps = x_pix_stride;
   p.q = (const unsigned char*)q8; p.s = s8; p.stats_in = stats;

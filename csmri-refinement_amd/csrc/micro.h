@@ -161,6 +161,11 @@ static inline dim3 row_walk_grid(long long rows, int slots, int unroll) {
   return dim3((unsigned)(gx < 1 ? 1 : gx), (unsigned)gy);
 }
 
+// Do two buffers of fp32 values share an element?  (Sums that add to one place from two threads would lose one another's.)
+static inline bool buffers_meet(const float* a, long long na, const float* b, long long nb) {
+  return a && b && a < b + nb && b < a + na;
+}
+
 // oa[col] (+)= sum over rows of partial[row][col] for col < na, ob[col] likewise for the nb columns behind them, in a fixed
 // order (act8.hip; the weight gradient's slabs and the layer norm's affine partials end in it)
 int micro_colsum2(const float* partial, int rows, long long row_stride, long long na, float* oa, long long nb, float* ob,

@@ -658,7 +658,8 @@ int csmri_ln_fwd(int dtype, const void* x, int x_pix_stride, void* z, int z_pix_
  * dgamma = sum_p dy h, dbeta = sum_p dy.  The input is either x (m and r are computed again) or q8 / s8 with the
  * forward's stats; with the kept form and slope != 1, z is needed for the sign of y, which it has where slope >= 0
  * (E_ARG below); optional otherwise.  dx may be
- * NULL; dgamma and dbeta (both or neither, [C_real], added to where accumulate != 0) need partial:
+ * NULL and must not overlap dz, x or z; dgamma and dbeta (both or neither, [C_real], apart from each other (E_ARG), added to
+ * where accumulate != 0) need partial:
  * [csmri_ln_bwd_rows(npix, C)][2][C_real] fp32, or any address where that is one row, which is not written.  Fixed
  * summation order. */
 int csmri_ln_bwd_rows(long long npix, int C);
@@ -679,7 +680,7 @@ int csmri_act8_restore(const void* q8, const uint8_t* s8, long long npix, int C,
                        void* stream);
 /* Weight gradient of a 1 x 1 stride-1 convolution whose input was kept in 8 bits (csmri_wgrad for that case):
  *   dw[n][c] (+)= sum_p dy[p][n] xhat[p][c],  db[n] (+)= sum_p dy[p][n]
- * dw: fp32 [Cout_real][Cin_real]; db: fp32 [Cout_real] or NULL; Cout, Cin: padded channel counts of dy and of the kept
+ * dw: fp32 [Cout_real][Cin_real]; db: fp32 [Cout_real], apart from dw (E_ARG), or NULL; Cout, Cin: padded channel counts of dy and of the kept
  * input.  The kept values enter the bf16 matrix instruction exactly; an fp32 dy is split into three bf16 parts,
  * without loss from 2^-103 up.
  * splits: csmri_act8_wgrad_splits; slab: csmri_act8_wgrad_slab_bytes (NULL when that is 0).  Fixed summation order.

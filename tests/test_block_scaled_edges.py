@@ -344,3 +344,44 @@ def test_kept_codes_with_the_smallest_and_the_nan_scale(ops):
   saved.kept = kept(nan)
   gx = ops.layer_norm_bwd(torch.ones(6, 64, device='cuda'), saved, z)[0].cpu()
   assert torch.isnan(gx[3]).all()
+
+
+# ---- outputs that meet ------------------------------------------------------------------------------------------------------
+def test_gradients_that_share_memory_are_refused(host_ops, monkeypatch):
+  """Two sums go to two places: threads that add to one would lose each other's."""
+  raw, p = host_ops.lib.raw, 1 << 20
+  bw, wg = raw('csmri_ln_bwd'), raw('csmri_act8_wgrad')
+  ln = lambda dg, db: bw(0, p, 16, 2 * p, 16, None, None, None, None, 0, 3 * p, 16, 4, 16, 13, 4 * p, 1e-5, 1.0, 5 * p, dg, db, 1, None)
+  for d in (0, 4, 48):
+    assert ln(6 * p, 6 * p + d) == -1 and ln(6 * p + d, 6 * p) == -1
+  act8 = lambda dw, db: wg(0, p, 16, 2 * p, 3 * p, 4, 16, 16, 13, 11, 1, None, dw, db, 1, None)
+  for dw, db in ((6 * p, 6 * p), (6 * p, 6 * p + 4 * 142), (6 * p + 48, 6 * p)):
+    assert act8(dw, db) == -1
+  # npix == 0 writes too
+  assert bw(0, None, 16, None, 16, None, None, None, None, 0, None, 16, 0, 16, 13, 4 * p, 1e-5, 1.0, 5 * p, 6 * p, 6 * p, 0, None) == -1
+  monkeypatch.setattr(host_ops, '_need_gpu', lambda t: None)
+  monkeypatch.setattr(host_ops.lib, 'call', lambda *a: pytest.fail('launched'))
+  x, flat = torch.zeros(4, 24), torch.zeros(64)
+  saved = host_ops.LNSaved(x, None, torch.zeros(48), (4, 24), torch.float32, 24, 1e-5, 1.0)
+  for dg, db in ((flat[:24], flat[:24]), (flat[:24], flat[23:47])):
+    with pytest.raises(ValueError):
+      host_ops.layer_norm_bwd(x, saved, dgamma=dg, dbeta=db)
+  kept = host_ops.Act8(torch.zeros(4, 8, dtype=torch.uint8), torch.zeros(4, 1, dtype=torch.uint8), (4, 8), torch.float32)
+  with pytest.raises(ValueError):
+    host_ops.act8_wgrad(kept, x, 5, 8, dw=flat[:40], db=flat[39:44])
+  p = torch.nn.Parameter(torch.ones(24))
+  with pytest.raises(ValueError):
+    host_ops.LayerNormAct.apply(x, p, p)
+
+
+@pytest.mark.gpu
+def test_gradients_side_by_side_are_written(ops):
+  x = torch.randn(9, 24, generator=torch.Generator().manual_seed(12)).cuda()
+  _, saved = ops.layer_norm(x, torch.ones(24, device='cuda'), torch.zeros(24, device='cuda'))
+  want, flat = ops.layer_norm_bwd(x, saved), torch.zeros(24 * 24 + 24, device='cuda')
+  ops.layer_norm_bwd(x, saved, dgamma=flat[24:48], dbeta=flat[:24])
+  assert torch.equal(flat[24:48], want[1]) and torch.equal(flat[:24], want[2]) and not flat[48:].any()
+  kept = ops.act8_save(x)
+  want = ops.act8_wgrad(kept, x)
+  ops.act8_wgrad(kept, x, dw=flat[:576], db=flat[576:])
+  assert torch.equal(flat[:576].view(24, 24), want[0]) and torch.equal(flat[576:], want[1])
