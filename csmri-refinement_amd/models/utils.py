@@ -199,6 +199,9 @@ def refresh_packs(model):
       if layer._bias_pad is not None:
         layer._bias_pad = (None, layer._bias_pad[1])
         layer.bias_padded()
+      if layer._pack4 is not None:
+        layer._pack4 = (None, layer._pack4[1])
+        layer._pack_mx4()
   for m in owners:
     ensure_pack_group(m).repack_stale()
 

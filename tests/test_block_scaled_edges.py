@@ -385,3 +385,32 @@ def test_gradients_side_by_side_are_written(ops):
   want = ops.act8_wgrad(kept, x)
   ops.act8_wgrad(kept, x, dw=flat[:576], db=flat[576:])
   assert torch.equal(flat[:576].view(24, 24), want[0]) and torch.equal(flat[576:], want[1])
+
+
+# ---- 4-bit copies of frozen layers -------------------------------------------------------------------------------------------
+def small_unet(seed):
+  from models import unet
+  torch.manual_seed(seed)
+  return unet.UNET(1, 1, 2, [32, 64], [32], 'none', kernel_size=3, upsampling_mode='nn-resize-conv', padding='reflection',
+                   decoder_act_upsampling_only=True, compute_dtype='bf16').cuda()
+
+
+@pytest.mark.gpu
+def test_frozen_4bit_layers_follow_loaded_weights(ops):
+  """refresh_packs reaches the 4-bit copies of frozen layers as it reaches their other packed ones, in place."""
+  from models import utils
+  x = torch.randn(2, 1, 64, 64, generator=torch.Generator().manual_seed(8)).cuda()
+  net, other = small_unet(5).eval(), small_unet(6).eval()
+  for m in (net, other):
+    assert utils.set_mx4_forward(m) == 1
+    utils.freeze(m)
+  with torch.no_grad():
+    first, want = net(x), other(x)
+    layer = net.head['0'].layer
+    assert layer._pack4 is not None and not torch.equal(first, want)
+    buf = layer._pack4[1].addresses()
+    net.load_state_dict(other.state_dict())
+    ops.bump_weight_epoch()
+    utils.refresh_packs(net)
+    assert torch.equal(net(x), want)
+    assert layer._pack4[1].addresses() == buf
