@@ -1220,11 +1220,25 @@ def _two_grads(ctx, g_a, g_b, dtype):
   return g_a, g_b
 
 
+class _ConvNode(torch.autograd.Function):
+  """Base of the convolution nodes.  A node's forward() runs with gradients off and cannot tell whether a graph is being
+  recorded around it; apply() can, and leaves it in ``recording``."""
+  recording = False
+
+  @classmethod
+  def apply(cls, *args):
+    outer, _ConvNode.recording = _ConvNode.recording, torch.is_grad_enabled()
+    try:
+      return super(_ConvNode, cls).apply(*args)
+    finally:
+      _ConvNode.recording = outer
+
+
 def _save_conv_inputs(ctx, layer, w_req, x0, x1, *rest):
   """save_for_backward of a convolution node: its inputs as they are, or in 8 bits (layer.keep8; only the weight
-  gradient reads them), and ``rest``."""
+  gradient reads them; not where no graph is recorded), and ``rest``."""
   ctx.kept = None
-  if layer.keep8 and w_req:
+  if layer.keep8 and w_req and _ConvNode.recording:
     kept = [None if t is None else act8_save(t) for t in (x0, x1)]
     ctx.kept = [None if a is None else (a.shape, a.dtype) for a in kept]
     ctx.save_for_backward(*([None if a is None else a.buf for a in kept] + list(rest)))
@@ -1241,7 +1255,7 @@ def _saved_conv_inputs(ctx):
   return tuple(x) + tuple(saved[2:])
 
 
-class ConvAct(torch.autograd.Function):
+class ConvAct(_ConvNode):
   """pad -> conv -> (+bias) -> LeakyReLU/ReLU, one kernel.  inputs: x0, x1|None,
   weight, bias (the Parameters, so autograd schedules the backward)."""
 
@@ -1634,7 +1648,7 @@ def _bn_forward(y, stats, bn, c_real, slope, training, dropmask, groups=1):
   return z, mean, invstd, snap
 
 
-class ConvBnAct(torch.autograd.Function):
+class ConvBnAct(_ConvNode):
   """pad -> conv(no bias) -> BatchNorm2d -> LeakyReLU -> channel dropout mask.
 
   The conv epilogue emits per-channel partial sums (no extra pass for the batch

@@ -414,3 +414,31 @@ def test_frozen_4bit_layers_follow_loaded_weights(ops):
     utils.refresh_packs(net)
     assert torch.equal(net(x), want)
     assert layer._pack4[1].addresses() == buf
+
+
+# ---- inference with layers that keep their inputs --------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_inputs_are_kept_only_where_a_backward_pass_can_follow(ops, monkeypatch):
+  from models import utils
+  calls = []
+  save = ops.act8_save
+  monkeypatch.setattr(ops, 'act8_save', lambda x: calls.append(x.shape) or save(x))
+  net = small_unet(5)
+  x = torch.randn(2, 1, 64, 64, generator=torch.Generator().manual_seed(8)).cuda()
+  n = utils.set_keep8(net)
+  with torch.no_grad():
+    net.eval()(x)
+    assert not calls
+    y = net.train()(x)
+    assert not calls
+    with torch.enable_grad():
+      z = net(x)
+    assert len(calls) >= n
+  assert torch.equal(y, z)
+  z.sum().backward()
+  assert all(p.grad is not None for p in net.parameters())
+  del calls[:]
+  for p in net.parameters():
+    p.requires_grad_(False)
+  net(x.requires_grad_(True))
+  assert not calls
