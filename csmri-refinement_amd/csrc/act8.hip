@@ -1,8 +1,8 @@
 // Activations kept for the backward pass in 8 bits (micro.h: e4m3 elements, one power-of-two scale per 32 channels of a
 // pixel: 1.03 bytes a channel instead of 2 or 4), and the weight gradient of a 1 x 1 convolution that reads them.
 //
-// Save and restore are streams: one read, one write, bound by HBM (16384 x 2048 bf16: 17 us for 102 MB; 131072 x 64: 6.7 and
-// 5.9 us for 25 MB, a third of it the launch).  A thread keeps its channels and has four rows under way.
+// Save and restore are streams: one read, one write, bound by HBM (16384 x 2048 bf16: 18 us for 102 MB; 131072 x 64: 6.1 and
+// 6.0 us for 25 MB, a third of it the launch).  A thread keeps its channels and has four rows under way.
 #include "micro.h"
 #include "wgrad_params.h"
 #include <type_traits>
@@ -208,9 +208,9 @@ __device__ __forceinline__ void split3(const float* f, u32x4_t* o) {
 // time.  Both operands pass through registers into one of two LDS stages, the input's codes becoming bf16 on the way, and
 // are loaded a step ahead of that.  (LDS-DMA would spare dY the registers, but the compiler lets no transposed read pass a
 // pending one; a second set of registers, to load two steps ahead, costs more in occupancy than it hides.)  Bound by the
-// matrix unit and the staging beside it: 165 - 177 us at 2048 x 2048 channels and 16384 pixels (800 TFLOP/s), where
-// the products alone take 109 at the clock they leave the chip, their fragment reads and barriers 20 - 28 more, and the loads
-// and staging the rest.  LDS is not what bounds it: images turned over in
+// matrix unit and the staging beside it: 165 us at 2048 x 2048 channels and 16384 pixels with the launch that adds the
+// splits' sums, back to back (830 TFLOP/s; in a kernel trace 188 + 15), where the products alone take 109 at the clock they
+// leave the chip, their fragment reads and barriers 20 - 28 more, and the loads and staging the rest.  LDS is not what bounds it: images turned over in
 // registers, [channel][pixel], and read 16 bytes at a time halve its reads and took 178.
 //
 // GK = 2: a second set of waves takes every other step, with stages of its own, and hands its sums over at the end -- the
@@ -420,8 +420,9 @@ __global__ __launch_bounds__(64 * WN * WC * GK, 2) void act8_wgrad_kernel(const 
 // Tile: 64 or 128 a side by the channel counts; 256 x 256 (an fp32 dY's three planes do not fit it), which reads LDS a third
 // less per product, where that leaves every CU 2304 pixels of a tile or more -- below, its larger partial sums cost as much
 // -- and covers no more than a tenth beyond what the smaller tiles do.
-// us with it and with 128 x 128, sums included: 16384 pixels, 2048 to 2048 184 / 199; 32768, 1024 to 2048 169 / 194;
-// 16384, 1536 to 1536 110 / 168; 65536, 512 to 1024 101 / 102; 24576, 1024 to 1024 84 / 79; 8192, 2048 to 2048 102 / 99.
+// us with it and with 128 x 128, sums included, back to back: 16384 pixels, 2048 to 2048 164 / 176; 32768, 1024 to 2048
+// 162 / 181; 16384, 1536 to 1536 109 / 170; 65536, 512 to 1024 100 / 99; 24576, 1024 to 1024 84 / 79; 8192, 2048 to 2048
+// 102 / 94.
 struct A8WTile { int bn, bc; };
 static A8WTile a8w_tile(int dy_dtype, long long npix, int Cout, int Cin) {
   const double big = (double)cdiv(Cout, 256) * cdiv(Cin, 256), small = (double)cdiv(Cout, 128) * cdiv(Cin, 128);

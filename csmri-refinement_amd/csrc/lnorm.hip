@@ -11,8 +11,10 @@
 // itself was kept in 8 bits (micro.h) the forward's m and r are stored next to it and the backward takes 1.03 bytes a
 // channel instead of 2 or 4.  dgamma and dbeta gather in registers over the rows a workgroup walks and leave as one
 // partial row per workgroup, summed in fixed order by a second launch: no atomics, the same bits on every run.
-// 8 x 256 x 256 x 32 bf16: 14 and 23 us, 4.8 and 4.4 TB/s, + 4 us for the sums; 8 x 64 x 64 x 1024 with the input kept in
-// 8 bits: 40 and 37 us, 4.2 and 4.6 TB/s, + 4 us; 64 fp32 pixels of 100 channels: 3.8 us.
+// 8 x 256 x 256 x 32 bf16: 15 and 24 us, 4.6 and 4.1 TB/s, + 4 us for the sums; 8 x 64 x 64 x 1024 with the input kept in
+// 8 bits: 41 and 37 us, 4.2 and 4.5 TB/s, + 5 us; 64 fp32 pixels of 100 channels: 3.9 us.  Behind a LeakyReLU the backward
+// also needs the sign of y: from x 8 x 256 x 256 x 32 takes 28 us, 8 x 64 x 64 x 1024 78 (41 without: beta is read again for
+// every row); from z, of an input kept in 8 bits, 44 (38 without) for 40 % more bytes.
 #include "micro.h"
 
 struct LNParams {

@@ -5,8 +5,12 @@
 //
 // A row of K channels is 64 bytes of codes per 128 channels (two a byte, the even channel in the low half) and one scale
 // byte per 32 channels, padded to 16 bytes per 512 channels; padding is code 0, scale 2^0.  The contraction is
-// v_mfma_scale_f32_16x16x128_f8f6f4: a lane's operand is 32 channels of one row, exactly one block, so its scale rides
-// in the lane next to it.  Products and sums are exact to fp32 (the elements are multiples of 1/2 up to 6).
+// v_mfma_scale_f32_*_f8f6f4, 16x16x128 for few rows and 32x32x64 in the tiles: a lane's operand is 32 channels of one row,
+// exactly one block, so its scale rides in the lane next to it.  Products are exact (the elements are multiples of 1/2 up
+// to 6); sums across blocks of different scales round to fp32.
+//
+// Times below: a kernel's own are medians of a kernel trace; where "back to back" is said, launches one behind the other
+// without one, which the large products run 10 - 15 % faster.
 #include "micro.h"
 
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
@@ -208,7 +212,7 @@ __device__ __forceinline__ void mx4_store(const MxParams& p, long long m, int n,
 }
 
 // Few rows (up to 16 MF): bound by the weights' bytes, and for one row by the latency of a single pass over them (1 x 4096
-// x 4096: 5.4 us, 8.9 MB; 64 x 4096 x 4096: 11 us).  A workgroup of eight waves owns 16 outputs; the waves split the
+// x 4096: 5.9 us, 4.8 on codes, 8.9 MB; 64 x 4096 x 4096: 12 us).  A workgroup of eight waves owns 16 outputs; the waves split the
 // channels, each lane reads its operands straight from memory, and the eight partial tiles are added in wave order.
 // QX: a lane quantises its own 32 channels of x, which saves the launch of a quantisation kernel.
 template <int MF, int QX>          // QX: -1 = x comes quantised, else the type of x
@@ -279,8 +283,9 @@ typedef __attribute__((ext_vector_type(16))) float f32x16_t;
 
 // Many rows: a workgroup of WM x WN waves takes 32 FM WM rows x 32 FN WN outputs.  Codes and scales reach LDS by LDS-DMA,
 // 256 channels a stage -- 128 bytes of a row, a cache line -- and two stages: one is read, the next one lands.
-// 16384 x 4096 x 4096: 157 - 165 us, 3.4 PFLOP/s at the 1.8 GHz that the chip holds under it; products and fragment reads
-// alone take 98, the loads add 30, the transposed stores of bf16 rows 27.  Workgroups that stay and store a tile under the
+// 16384 x 4096 x 4096: 161 us back to back, 3.4 PFLOP/s at the 1.8 GHz that the chip holds under it (187 in a trace of it
+// behind its quantisation, 167 on codes); products and fragment reads alone take 98, the loads add 30, the transposed
+// stores of bf16 rows 27: time that nothing overlaps, not a bound.  8192^3: 295 us back to back, 3.7 PFLOP/s.  Workgroups that stay and store a tile under the
 // next one's products, halves of a workgroup that take turns, and fragments read a quarter of a step ahead took as long.
 // The 32 x 32 x 64 form of the matrix instruction, not the 16 x 16 x 128 one: both take the scale operands in an
 // instruction slot of their own, which costs the shorter one more of its rate (a loop of nothing else reaches 9.5
@@ -343,7 +348,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void mx4_gemm_kernel(const MxPar
   const int tz = xcd_remap(blockIdx.x, p.mtiles * p.ntiles * p.splits), split = tz / (p.mtiles * p.ntiles);
   const int t = tz - split * p.mtiles * p.ntiles;
   // bands of eight row tiles: what runs on an XCD at one time is about square and shares its operands in L2
-  // (8192^3: 309 us, 318 in row order; 16384 x 4096 x 4096: 186, 192; smaller ones alike)
+  // (8192^3 and 16384 x 4096 x 4096 take 3 % longer in row order; smaller ones as long)
   const int band = t / (8 * p.ntiles), r = t - band * 8 * p.ntiles, bm = min(8, p.mtiles - band * 8);
   const int mt = band * 8 + r % bm, nt = r / bm, k0 = split * p.schunk;
   const long long m0 = (long long)mt * BM; const int n0 = nt * BN;
@@ -519,8 +524,9 @@ static int mx4_splits(long long rows, int K, int N) {
 }
 // The 256 x 256 tile reads each operand half as often and has a CU to itself; two of the 128 x 128 ones share one.  At 4096
 // channels a round of 256 large tiles takes 40 us, 512 small ones 24 us and 6 us for the first and last, and those need
-// not come in whole rounds.  us with large tiles and with small ones: 16384 x 4096 x 4096 157 / 183, 4096^3 43 / 50,
-// 3584 x 4096 x 4096 40 / 49; 2048 x 4096 x 4096 37 / 30, 16384 x 2048 x 1100 41 / 35, 131072 x 512 x 128 26 / 18.
+// not come in whole rounds.  us with large tiles and with small ones, back to back: 16384 x 4096 x 4096 161 / 191, 8192^3
+// 294 / 360, 4096^3 42 / 49, 3584 x 4096 x 4096 39 / 45; 2048 x 4096 x 4096 34 / 26, 16384 x 2048 x 1100 41 / 33,
+// 131072 x 512 x 128 24 / 17.
 static bool mx4_large(long long rows, int N) {
   const long long small = ((rows + 127) / 128) * ((N + 127LL) / 128), big = ((rows + 255) / 256) * ((N + 255LL) / 256);
   return 40 * 512 * ((big + 255) / 256) < 6 * 512 + 24 * small;

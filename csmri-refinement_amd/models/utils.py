@@ -60,14 +60,19 @@ def _set_layer_flag(module, name, on, wanted):
 
 def set_mx4_forward(module, on=True):
   """Switch the 4-bit forward products of every trainable 1 x 1 convolution under ``module`` (ops.ConvLayer.mx4); returns
-  how many layers that concerns.  Gradients are those of the 16- or 32-bit path, through the rounding."""
+  how many layers that concerns.  Gradients are those of the 16- or 32-bit path, through the rounding.
+  It pays for wide layers (16384 pixels of 4096 -> 4096 channels: 202 us, bf16 566; 32768 of 1024 -> 1024: 50, 77) and costs
+  for narrow ones, whose padded 4-bit rows are no smaller: the U-Net's 32 -> 1 head is such a one (524288 pixels of 32 -> 2:
+  54, 14.5)."""
   return _set_layer_flag(module, 'mx4', on, lambda layer: layer.pointwise())
 
 
 def set_keep8(module, on=True):
   """Keep the inputs of every trainable convolution under ``module`` in 8 bits for their weight gradients
   (ops.ConvLayer.keep8); returns how many layers that concerns.  Outputs and data gradients do not change.  Conv blocks
-  that run as one launch and replayed sub-batches keep theirs as they are: those inputs are held for other reasons."""
+  that run as one launch and replayed sub-batches keep theirs as they are: those inputs are held for other reasons.
+  Memory for time: a bf16 U-Net of 32 and 64 channels on 8 x 256 x 256 holds 330 MB between its passes instead of 434 and
+  takes 2.05 ms for both instead of 1.76 (3 x 3 layers restore their inputs; 1 x 1 ones read the codes, faster than bf16)."""
   return _set_layer_flag(module, 'keep8', on, lambda layer: True)
 
 
