@@ -430,7 +430,7 @@ def quantize_fp8(x, amax=None):
 # block-scaled formats: kept activations (8 bits), 4-bit rows, layer norm
 # ----------------------------------------------------------------------------
 # These take tensors [..., C] of any leading shape, their last axis the channels of a pixel (C a multiple of 8, pad
-# channels zero), strided pixels included; what the kernels cannot address (a strided channel axis, a pointer or pixel
+# channels zero), strided pixels included; what the kernels cannot address (a strided channel axis, broadcast pixels, a pointer or pixel
 # stride that is no multiple of 16 bytes) is copied first.  They launch on the current stream of the tensor's device.
 
 
@@ -1220,25 +1220,25 @@ def _two_grads(ctx, g_a, g_b, dtype):
   return g_a, g_b
 
 
-class _ConvNode(torch.autograd.Function):
-  """Base of the convolution nodes.  A node's forward() runs with gradients off and cannot tell whether a graph is being
-  recorded around it; apply() can, and leaves it in ``recording``."""
+class _Node(torch.autograd.Function):
+  """Base of the nodes that can keep an input in 8 bits.  A node's forward() runs with gradients off and cannot tell whether
+  a graph is being recorded around it; apply() can, and leaves it in ``recording``."""
   recording = False
 
   @classmethod
-  def apply(cls, *args):
-    outer, _ConvNode.recording = _ConvNode.recording, torch.is_grad_enabled()
+  def apply(cls, *args, **kwargs):
+    outer, _Node.recording = _Node.recording, torch.is_grad_enabled()
     try:
-      return super(_ConvNode, cls).apply(*args)
+      return super(_Node, cls).apply(*args, **kwargs)
     finally:
-      _ConvNode.recording = outer
+      _Node.recording = outer
 
 
 def _save_conv_inputs(ctx, layer, w_req, x0, x1, *rest):
   """save_for_backward of a convolution node: its inputs as they are, or in 8 bits (layer.keep8; only the weight
   gradient reads them; not where no graph is recorded), and ``rest``."""
   ctx.kept = None
-  if layer.keep8 and w_req and _ConvNode.recording:
+  if layer.keep8 and w_req and _Node.recording:
     kept = [None if t is None else act8_save(t) for t in (x0, x1)]
     ctx.kept = [None if a is None else (a.shape, a.dtype) for a in kept]
     ctx.save_for_backward(*([None if a is None else a.buf for a in kept] + list(rest)))
@@ -1255,7 +1255,7 @@ def _saved_conv_inputs(ctx):
   return tuple(x) + tuple(saved[2:])
 
 
-class ConvAct(_ConvNode):
+class ConvAct(_Node):
   """pad -> conv -> (+bias) -> LeakyReLU/ReLU, one kernel.  inputs: x0, x1|None,
   weight, bias (the Parameters, so autograd schedules the backward)."""
 
@@ -1648,7 +1648,7 @@ def _bn_forward(y, stats, bn, c_real, slope, training, dropmask, groups=1):
   return z, mean, invstd, snap
 
 
-class ConvBnAct(_ConvNode):
+class ConvBnAct(_Node):
   """pad -> conv(no bias) -> BatchNorm2d -> LeakyReLU -> channel dropout mask.
 
   The conv epilogue emits per-channel partial sums (no extra pass for the batch
@@ -1751,8 +1751,9 @@ class ConvBnAct(_ConvNode):
     return gx0, gx1, None, None, None, None, None, None, None, None, None
 
 
-class LayerNormAct(torch.autograd.Function):
-  """layer_norm as an autograd node: z = lrelu(layer norm of x over its channels).  ``keep8``: x is kept in 8 bits.
+class LayerNormAct(_Node):
+  """layer_norm as an autograd node: z = lrelu(layer norm of x over its channels).  ``keep8``: x is kept in 8 bits, where a
+  graph is recorded.
   Like the BatchNorm node's, the affine gradients are accumulated into gamma.grad / beta.grad by the kernels, so the two
   have to be leaves (Parameters)."""
 
@@ -1762,11 +1763,14 @@ class LayerNormAct(torch.autograd.Function):
       raise ValueError('csmri_hip: LayerNormAct writes the gradients of gamma and beta itself: they have to be leaf tensors')
     if gamma is beta:
       raise ValueError('csmri_hip: LayerNormAct needs two tensors for gamma and beta: their gradients are written at once')
+    if slope < 0 and keep8:
+      raise ValueError('csmri_hip: LayerNormAct with keep8 needs a slope of 0 or more')
+    keep8 = bool(keep8) and _Node.recording and any(ctx.needs_input_grad)
     z, sv = layer_norm(x, gamma, beta, eps, slope, keep8)
     ctx.gamma, ctx.beta = gamma, beta
     ctx.affine_req = (gamma.requires_grad, beta.requires_grad)
     ctx.meta = (sv.shape, sv.dtype, sv.c_real, sv.eps, sv.slope)
-    ctx.keep8 = bool(keep8)
+    ctx.keep8 = keep8
     if keep8:
       ctx.save_for_backward(sv.kept.buf, sv.aux, z if slope != 1.0 else None)
     else:

@@ -442,3 +442,24 @@ def test_inputs_are_kept_only_where_a_backward_pass_can_follow(ops, monkeypatch)
     p.requires_grad_(False)
   net(x.requires_grad_(True))
   assert not calls
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('slope', [1.0, 0.2])
+def test_layer_norm_node_keeps_its_input_only_where_a_backward_pass_can_follow(ops, monkeypatch, slope):
+  asked = []
+  norm = ops.layer_norm
+  monkeypatch.setattr(ops, 'layer_norm', lambda *a: asked.append(bool(a[5])) or norm(*a))
+  x = torch.randn(33, 72, generator=torch.Generator().manual_seed(9)).cuda()
+  ga, be = torch.nn.Parameter(torch.linspace(0.5, 1.5, 72).cuda()), torch.nn.Parameter(torch.linspace(-1, 1, 72).cuda())
+  node = lambda x, ga, be: ops.LayerNormAct.apply(x, ga, be, 1e-5, slope, True)
+  with torch.no_grad():
+    a = node(x, ga, be)
+    b = node(x.requires_grad_(True), ga, be)
+  x = x.detach()
+  c = node(x, ga.detach(), be.detach())
+  assert asked == [False] * 3 and torch.equal(a, b) and torch.equal(a, c)
+  z = node(x, ga, be)
+  assert asked[3:] == [True] and torch.equal(z, a)
+  z.sum().backward()
+  assert ga.grad is not None and be.grad is not None
