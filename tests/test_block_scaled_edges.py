@@ -463,3 +463,24 @@ def test_layer_norm_node_keeps_its_input_only_where_a_backward_pass_can_follow(o
   assert asked[3:] == [True] and torch.equal(z, a)
   z.sum().backward()
   assert ga.grad is not None and be.grad is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('multi', ['0', '1', 'auto'])
+@pytest.mark.parametrize('defer', [0, 2])
+def test_both_kinds_of_weight_gradient_on_the_side_stream(ops, monkeypatch, multi, defer):
+  """The same with the weight gradients on their own stream, issued at once or held back."""
+  backward = torch.autograd.backward
+
+  def joined(*args):
+    backward(*args)
+    ops.join_wgrad_stream()
+  monkeypatch.setattr(torch.autograd, 'backward', joined)
+  monkeypatch.setattr(ops, 'WGRAD_DEFER', defer)
+  ops.enable_wgrad_stream(True)
+  try:
+    for keeps in ((True, False), (False, True), (False, True, False)):
+      for fresh in (False, True):
+        test_layer_used_with_kept_and_with_plain_inputs_in_one_backward(ops, monkeypatch, multi, keeps, fresh)
+  finally:
+    ops.enable_wgrad_stream(False)
